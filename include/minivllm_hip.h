@@ -155,6 +155,36 @@ int mvllm_paged_attention(void* out, const void* q, const void* key_pool,
                           int32_t kv_dtype, const mvllm_plan_options* options, void* workspace,
                           uint64_t workspace_bytes, void* stream);
 
+/* mvllm_paged_attention over a sliding window with sinks: a query at position p (query r of a
+ * sequence: S - L + r) sees the keys j <= p with j > p - window or j < sinks: the `window` newest
+ * ones, itself among them, and the sequence's `sinks` first. No counterpart in the reference.
+ * Arguments, types and head dims as mvllm_paged_attention, the plan from
+ * mvllm_paged_window_attention_plan with the same window and sinks; window >= 1, sinks >= 0 (either
+ * may be larger than any context), max_context_len < 2^30 - 4096, context_lens[s] >= seq_lens[s].
+ *   A page holding no key that a query of the call sees is not read and its table entry may be
+ * anything (-1: a rolling cache gives such pages to other sequences), and what the keys that no
+ * query sees hold in a page that is read has no part in the result. K and V of a key that some
+ * query sees must be finite. A decode row without a key (context_lens[s] <= 0) is zeros; rows of
+ * out that belong to no sequence are left as they are. */
+int mvllm_paged_window_attention_plan(int32_t num_tokens, int32_t num_seqs, int32_t num_q_heads,
+                                      int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                      int32_t max_query_len, int32_t max_context_len,
+                                      int32_t window, int32_t sinks, int32_t q_dtype,
+                                      int32_t kv_dtype, const mvllm_plan_options* options,
+                                      mvllm_paged_plan* plan);
+int mvllm_paged_window_attention(void* out, const void* q, const void* key_pool,
+                                 const void* value_pool, const float* k_scales,
+                                 const float* v_scales, const int32_t* block_tables,
+                                 const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                                 const int32_t* seq_lens, int32_t num_tokens, int32_t num_seqs,
+                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t block_size, int64_t num_blocks,
+                                 int32_t max_blocks_per_seq, int32_t max_query_len,
+                                 int32_t max_context_len, int32_t window, int32_t sinks,
+                                 float scale, int32_t q_dtype, int32_t kv_dtype,
+                                 const mvllm_plan_options* options, void* workspace,
+                                 uint64_t workspace_bytes, void* stream);
+
 /* mvllm_paged_attention for callers that cannot allocate device memory (code under
  * HIP graph capture, tight serving loops, harnesses that forbid hipMalloc); no
  * counterpart in the reference. The same arguments without the workspace: the split

@@ -236,14 +236,15 @@ struct PairWork {
   int64_t n;      // key tiles of the longest item, at most (a decode row's context may be longer)
   int64_t tiles;  // of all items, with the longest's context
 };
-PairWork pair_work(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t max_q, int32_t max_ctx) {
+// `span` bounds the keys that an item walks: the context, or a windowed item's list.
+PairWork pair_work(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t max_q, int32_t span, bool windowed) {
   PairWork w{};
   const int64_t beyond = static_cast<int64_t>(num_tokens) - num_seqs;
   w.chunks = max_q > 1 && beyond > 0 ? (beyond + max_q - 2) / (max_q - 1) : 0;
   w.tokens = w.chunks > 0 ? beyond + w.chunks : 0;
   w.wgs = (w.tokens + 63) / 64 * (hq / 2);
-  w.n = (static_cast<int64_t>(max_ctx) + mvllm::kPrefillKeyTile - 1) / mvllm::kPrefillKeyTile;
-  w.tiles = w.wgs * (2 * w.n - max_q / 64) / 2;
+  w.n = (static_cast<int64_t>(span) + mvllm::kPrefillKeyTile - 1) / mvllm::kPrefillKeyTile;
+  w.tiles = windowed ? w.wgs * w.n : w.wgs * (2 * w.n - max_q / 64) / 2;
   return w;
 }
 
@@ -318,6 +319,12 @@ void plan_whole(Plan& plan, const PairWork& w, int32_t num_tokens, int32_t num_s
   }
 }
 
+// The window of a windowed call (0: every key is visible).
+struct Window {
+  int32_t window = 0;
+  int32_t sinks = 0;
+};
+
 // The MFMA prefill's schedule, from host sizes: the grid where its 128-query items, ceil(
 // num_tokens / 128) query tiles per kv column, reach half the CU count, the stream schedule
 // (balanced shares of all key tiles) below; the prefill_schedule option 1 / 2 forces
@@ -329,14 +336,22 @@ void plan_whole(Plan& plan, const PairWork& w, int32_t num_tokens, int32_t num_s
 // 8K-16K contexts).
 void plan_prefill(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk,
                   int32_t d, int32_t block_size, int32_t max_q, int32_t max_ctx, int32_t q_dtype,
-                  int32_t kv_dtype, const Options& o) {
+                  int32_t kv_dtype, const Options& o, const Window& win) {
   if (!plan.pub.prefill_mfma) return;
   plan.register_staging = o.prefill_staging;
   plan.prefill_share_tiles = o.prefill_share_tiles;
   const int forced = o.prefill_schedule;
   const int cus = device_cus();
   const bool pair = pair_prefill(hq, hk, d, block_size, q_dtype, kv_dtype, o);
-  const PairWork work = pair_work(num_tokens, num_seqs, hq, max_q, max_ctx);
+  const bool windowed = win.window > 0;
+  int64_t span = max_ctx;
+  if (windowed) {
+    // The sinks, a window and the item's queries, with the runs of 16 that they begin and end in.
+    const int64_t list = static_cast<int64_t>(win.sinks) + 15 + win.window + 15 + 63;
+    if (list < span) span = list;
+    if (!pair) return;  // (the other kernels run windowed items whole, on the item grid)
+  }
+  const PairWork work = pair_work(num_tokens, num_seqs, hq, max_q, static_cast<int32_t>(span), windowed);
   const PairMode m = pair_mode(work, num_seqs, hq, max_q, kv_dtype, cus);
   const int64_t qtiles = (static_cast<int64_t>(num_tokens) + mvllm::kPrefillQueryTile - 1) /
                          mvllm::kPrefillQueryTile;
@@ -381,12 +396,13 @@ void plan_prefill(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, 
 
 Plan make_plan(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int32_t d,
                int32_t block_size, int32_t max_q, int32_t max_ctx, int32_t q_dtype,
-               int32_t kv_dtype, const Options& o = Options{}) {
+               int32_t kv_dtype, const Options& o = Options{}, const Window& win = Window{}) {
   Plan plan{};
-  plan_decode(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, max_ctx, q_dtype,
-              kv_dtype, o);
+  // A single query's keys: its context, or its windowed list.
+  const int32_t keys = win.window > 0 ? mvllm::window_keys(max_ctx, win.window, win.sinks) : max_ctx;
+  plan_decode(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, keys, q_dtype, kv_dtype, o);
   plan_prefill(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, max_ctx, q_dtype, kv_dtype,
-               o);
+               o, win);
   if (plan.pub.prefill_mfma && pair_prefill(hq, hk, d, block_size, q_dtype, kv_dtype, o)) {
     plan.pub.prefill_item = plan.split_tile;
     plan.pub.prefill_listed = plan.split_pieces;
@@ -498,7 +514,7 @@ int launch_planned(const Plan& plan, mvllm::PagedParams& p, void* workspace, int
   }
   p.pf_tile = plan.split_tile;
   p.pf_pieces = plan.split_pieces;
-  if (plan.split_pieces > 1 && plan.pub.prefill_workgroups == 0) {
+  if (plan.split_pieces > 1 && plan.pub.prefill_workgroups == 0 && p.window == 0) {
     // The grid's cut items run whole under graph capture, counted: what callers of
     // mvllm_split_stats were promised when cutting needed counters of a stream's own. (The
     // cut needs none now, and the stream schedule's is captured as it is.)
@@ -736,7 +752,8 @@ int paged_attention_entry(const char* name, void* out, const void* q, const void
                           int64_t num_blocks, int32_t max_blocks_per_seq, int32_t max_query_len,
                           int32_t max_context_len, float scale, int32_t q_dtype,
                           int32_t kv_dtype, const mvllm_plan_options* options, void* workspace,
-                          uint64_t workspace_bytes, void* stream, bool static_scratch) {
+                          uint64_t workspace_bytes, void* stream, bool static_scratch,
+                          const Window& win = Window{}) {
   int rc = check_paged_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim,
                              block_size, max_query_len, max_context_len, q_dtype, kv_dtype);
   if (rc != MVLLM_OK) return rc;
@@ -760,7 +777,7 @@ int paged_attention_entry(const char* name, void* out, const void* q, const void
                 "only for one");
   }
   Plan plan = make_plan(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
-                        max_query_len, max_context_len, q_dtype, kv_dtype, o);
+                        max_query_len, max_context_len, q_dtype, kv_dtype, o, win);
   if (static_scratch && plan.pub.workspace_bytes > workspace_bytes && plan.pub.prefill_pieces > 1) {
     // The cut items' partial slots do not fit the static scratch: items stay whole.
     o.prefill_pieces = 1;
@@ -813,8 +830,29 @@ int paged_attention_entry(const char* name, void* out, const void* q, const void
   p.kv_head_bytes = static_cast<int64_t>(head_dim) * kv_elem;
   p.kv_row_bytes = p.kv_head_bytes * num_kv_heads;
   p.scale = scale;
+  p.window = win.window;
+  p.sinks = win.sinks;
   return launch_planned(plan, p, workspace, q_dtype, kv_dtype, head_dim, max_query_len,
                         static_cast<hipStream_t>(stream), name);
+}
+
+// The arguments of a windowed call: refusals, and the window as the kernels take it. (Capped
+// at 2^30, past every context served, so that sums of two stay in 32 bits.)
+constexpr int32_t kMaxWindow = 1 << 30;
+int read_window(int32_t window, int32_t sinks, int32_t max_context_len, Window& out) {
+  if (window < 1 || sinks < 0) {
+    return fail(MVLLM_ERR_INVALID,
+                "paged_window_attention: window must be >= 1 (a query sees itself) and sinks >= 0, "
+                "got %d and %d",
+                window, sinks);
+  }
+  if (max_context_len > kMaxWindow - 4096) {
+    return fail(MVLLM_ERR_UNSUPPORTED, "paged_window_attention: contexts of %d keys are not served",
+                max_context_len);
+  }
+  out.window = window < kMaxWindow ? window : kMaxWindow;
+  out.sinks = sinks < kMaxWindow - 64 ? sinks : kMaxWindow - 64;
+  return MVLLM_OK;
 }
 
 // The allocation-free entry's scratch: one array per device, held from the library's
@@ -872,6 +910,53 @@ int mvllm_paged_attention(void* out, const void* q, const void* key_pool,
                                block_size, num_blocks, max_blocks_per_seq, max_query_len,
                                max_context_len, scale, q_dtype, kv_dtype, options, workspace,
                                workspace_bytes, stream, false);
+}
+
+int mvllm_paged_window_attention_plan(int32_t num_tokens, int32_t num_seqs, int32_t num_q_heads,
+                                      int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                      int32_t max_query_len, int32_t max_context_len,
+                                      int32_t window, int32_t sinks, int32_t q_dtype,
+                                      int32_t kv_dtype, const mvllm_plan_options* options,
+                                      mvllm_paged_plan* plan) {
+  g_error[0] = '\0';
+  if (plan == nullptr) return fail(MVLLM_ERR_INVALID, "paged_window_attention_plan: plan is NULL");
+  int rc = check_paged_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                             block_size, max_query_len, max_context_len, q_dtype, kv_dtype);
+  if (rc != MVLLM_OK) return rc;
+  Options o;
+  rc = read_options(options, o);
+  if (rc != MVLLM_OK) return rc;
+  Window win;
+  rc = read_window(window, sinks, max_context_len, win);
+  if (rc != MVLLM_OK) return rc;
+  *plan = make_plan(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+                    max_query_len, max_context_len, q_dtype, kv_dtype, o, win)
+              .pub;
+  return MVLLM_OK;
+}
+
+int mvllm_paged_window_attention(void* out, const void* q, const void* key_pool,
+                                 const void* value_pool, const float* k_scales,
+                                 const float* v_scales, const int32_t* block_tables,
+                                 const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                                 const int32_t* seq_lens, int32_t num_tokens, int32_t num_seqs,
+                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t block_size, int64_t num_blocks,
+                                 int32_t max_blocks_per_seq, int32_t max_query_len,
+                                 int32_t max_context_len, int32_t window, int32_t sinks,
+                                 float scale, int32_t q_dtype, int32_t kv_dtype,
+                                 const mvllm_plan_options* options, void* workspace,
+                                 uint64_t workspace_bytes, void* stream) {
+  g_error[0] = '\0';
+  Window win;
+  const int rc = read_window(window, sinks, max_context_len, win);
+  if (rc != MVLLM_OK) return rc;
+  return paged_attention_entry("paged_window_attention", out, q, key_pool, value_pool, k_scales,
+                               v_scales, block_tables, cu_seqlens_q, context_lens, seq_lens,
+                               num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                               block_size, num_blocks, max_blocks_per_seq, max_query_len,
+                               max_context_len, scale, q_dtype, kv_dtype, options, workspace,
+                               workspace_bytes, stream, false, win);
 }
 
 int mvllm_paged_attention_noalloc(void* out, const void* q, const void* key_pool,

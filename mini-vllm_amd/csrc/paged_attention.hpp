@@ -218,7 +218,18 @@ struct PagedParams {
   float* pf_part;     // cut: [pf_slots][columns] partials of pair_slot_floats
   int4* pf_rec;       // [pf_ranks][2], each position's piece: for the merge, and from the
                       // schedule kernel (more than 64 sequences)
+  int window;         // > 0: windowed attention (the kernels' kWindow forms): a query at
+  int sinks;          // position p sees the keys j <= p with j > p - window or j < sinks
+                      // (sinks + window < 2^31)
 };
+
+// Windowed attention. The keys that the queries of a work item see are the sinks and one range
+// that ends at the last query's position, so an item walks them as a list without the keys
+// between: entry v is position v for v < front, v + gap from there on. A single query's list
+// holds exactly the keys it sees, this many of its `visible`.
+__host__ __device__ inline int window_keys(int visible, int window, int sinks) {
+  return visible < window + sinks ? visible : window + sinks;
+}
 
 // Splits of one row: as many as its visible context needs at `split_tokens` keys
 // each, never more than the grid provides. Shared by the decode kernel, the merge

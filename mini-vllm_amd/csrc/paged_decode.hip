@@ -96,6 +96,17 @@ __device__ __forceinline__ bool resolve_row(const PagedParams& p, int index, int
   return visible > 0;
 }
 
+// The same for windowed attention, whose rows without a key are zeros: true for every row that is
+// this pass's to write, `visible` then at most 0 where it has none. (By row: not the rows of q
+// behind the last sequence.)
+__device__ __forceinline__ bool resolve_window_row(const PagedParams& p, int index, int& seq, int& row,
+                                                   int& visible) {
+  if (resolve_row(p, index, seq, row, visible)) {
+    return !p.by_row || row - p.cu_seqlens_q[seq] < p.seq_lens[seq];
+  }
+  return p.by_row ? row - p.cu_seqlens_q[seq] < p.seq_lens[seq] : p.seq_lens[seq] == 1;
+}
+
 // One lane's E elements of a query head, and their dot product with a 16-byte chunk of a K
 // row in fp32. 16-bit queries stay packed and use the two-element dot instruction (exact
 // products, one rounding per pair: against 64 bits 1.27e-8 where the multiply-adds of widened
@@ -177,6 +188,16 @@ template <> struct Query<f16_t, f16_t> : PackedQuery<f16_t, f16_t> {};
 template <> struct Query<bf16_t, fp8_t> : PackedQuery<bf16_t, fp8_t> {};
 template <> struct Query<f16_t, fp8_t> : PackedQuery<f16_t, fp8_t> {};
 
+// Where the entries of a sequence's key list lie: all positions in order, or for windowed
+// attention the sinks and then, `gap` positions on, the window's keys.
+struct EveryKey {
+  __device__ int operator()(int v) const { return v; }
+};
+struct WindowKeys {
+  int sinks, gap;
+  __device__ int operator()(int v) const { return v < sinks ? v : v + gap; }
+};
+
 // Per-wave online-softmax state over a run of keys, for GC query heads.
 template <int GC, int E>
 struct WaveState {
@@ -225,7 +246,15 @@ struct Decode {
                                 const Q (&qf)[GC], float score_scale, State& st) {
     const Fresh none{-1, {}, {}};
     stream_with<false>(p, table, dense_base, lds_pages, first_page, kvh, sb, se, g, r, qf, score_scale, st,
-                       [] {}, none);
+                       [] {}, none, EveryKey{});
+  }
+
+  // The same over entries [sb, se) of a windowed sequence's key list.
+  __device__ static void stream_window(const PagedParams& p, const int32_t* table, const WindowKeys& keys,
+                                       int kvh, int sb, int se, int g, int r, const Q (&qf)[GC],
+                                       float score_scale, State& st) {
+    const Fresh none{-1, {}, {}};
+    stream_with<false>(p, table, 0, nullptr, 0, kvh, sb, se, g, r, qf, score_scale, st, [] {}, none, keys);
   }
 
   // The new token of a fresh-token stream: token `tok` of the run (< 0: none) takes this
@@ -240,11 +269,12 @@ struct Decode {
   // qf and `fresh`, so that arithmetic overlaps those loads), and with kFresh the step
   // holding fresh.tok takes that token's rows from `fresh`. (Forming them under the
   // first step's K/V requests instead measured the same, with 60% more registers.)
-  template <bool kFresh, typename Prep>
+  // `at` gives the position of an entry of the run.
+  template <bool kFresh, typename Prep, typename Keys>
   __device__ static void stream_with(const PagedParams& p, const int32_t* table,
                                      int dense_base, const int* lds_pages, int first_page, int kvh, int sb, int se,
                                      int g, int r, const Q (&qf)[GC], float score_scale,
-                                     State& st, Prep&& prep, const Fresh& fresh) {
+                                     State& st, Prep&& prep, const Fresh& fresh, const Keys& at) {
     static_assert(!(kFresh && kFp8), "the fresh-token stream serves 16-bit pools");
     const char* kbase = static_cast<const char*>(p.k_pool);
     const char* vbase = static_cast<const char*>(p.v_pool);
@@ -253,7 +283,7 @@ struct Decode {
 
     auto page_of = [&](int tok) -> int {
       if (table == nullptr) return dense_base + (tok & ~p.block_mask);
-      const int pi = tok >> p.block_shift;
+      const int pi = at(tok) >> p.block_shift;
       return lds_pages != nullptr ? lds_pages[pi - first_page] : table[pi];
     };
 
@@ -271,7 +301,7 @@ struct Decode {
         int tok = t0 + u * RG + g;
         valid[u] = tok < se;
         tok = valid[u] ? tok : se - 1;
-        const int64_t slot = (static_cast<int64_t>(pg[u]) << p.table_shift) + (tok & p.block_mask);
+        const int64_t slot = (static_cast<int64_t>(pg[u]) << p.table_shift) + (at(tok) & p.block_mask);
         const int64_t off = slot * p.kv_row_bytes + kvh * p.kv_head_bytes + r * E * kElemBytes;
         kw[u] = load16_stream(kbase + off);
         vw[u] = load16_stream(vbase + off);
@@ -424,7 +454,10 @@ __device__ __forceinline__ bool wave_unit(const PagedParams& p, int unit, int& k
 
 // kFresh: every sequence's last key is the step's new token, formed here from the
 // projection's output (FreshParams) instead of read from the pool.
-template <typename TQ, typename TKV, int D, int GC, bool kFresh>
+// kWindow: a sequence's keys are the entries of its windowed list (WindowKeys), at most window +
+// sinks of them whatever its context: the same loop over fewer keys, no key read for nothing and
+// no mask, with two instructions an entry more for its position.
+template <typename TQ, typename TKV, int D, int GC, bool kFresh, bool kWindow>
 __global__ __launch_bounds__(512) void paged_decode_stream_kernel(const PagedParams p,
                                                                   const FreshParams f) {
   using K = Decode<TQ, TKV, D, GC>;
@@ -440,11 +473,14 @@ __global__ __launch_bounds__(512) void paged_decode_stream_kernel(const PagedPar
   // A dense cache: every sequence holds dense_keys, nothing is read.
   const bool dense = !kFresh && p.dense_keys > 0;
   const bool by_lane = n <= kWave;
+  auto listed = [&](int context) __attribute__((always_inline)) -> int {
+    return kWindow ? window_keys(max(context, 0), p.window, p.sinks) : max(context, 0);
+  };
   int upto = 0;
   if (dense) {
   } else if (by_lane) {
     const int s = tid % kWave;
-    upto = wave_inclusive_scan(s < n && p.seq_lens[s] == 1 ? max(p.context_lens[s], 0) : 0);
+    upto = wave_inclusive_scan(s < n && p.seq_lens[s] == 1 ? listed(p.context_lens[s]) : 0);
   } else {
     // Each wave its run of sequences, 64 at a time: their sum, then their places after the
     // runs before.
@@ -455,7 +491,7 @@ __global__ __launch_bounds__(512) void paged_decode_stream_kernel(const PagedPar
     const int per = (n + blockDim.x - 1) / blockDim.x * kWave;
     const int first = min(w * per, n), end = min(first + per, n);
     auto keys = [&](int s) __attribute__((always_inline)) -> int {
-      return s < end && p.seq_lens[s] == 1 ? max(p.context_lens[s], 0) : 0;
+      return s < end && p.seq_lens[s] == 1 ? listed(p.context_lens[s]) : 0;
     };
     int run = 0;
 #pragma unroll 4
@@ -620,11 +656,16 @@ __global__ __launch_bounds__(512) void paged_decode_stream_kernel(const PagedPar
           }
         };
         K::template stream_with<true>(p, table, 0, nullptr, 0, kvh, sb, se, g, r, qf, score_scale,
-                                      st, prep, fresh);
+                                      st, prep, fresh, EveryKey{});
       } else {
         K::load_queries(p, row, h0, r, qf);
-        K::stream(p, dense ? nullptr : table, seq * p.dense_slots, nullptr, 0, kvh, sb, se, g, r, qf,
-                  score_scale, st);
+        if constexpr (kWindow) {
+          const WindowKeys keys{p.sinks, sload(p.context_lens + seq) - ctx};
+          K::stream_window(p, table, keys, kvh, sb, se, g, r, qf, score_scale, st);
+        } else {
+          K::stream(p, dense ? nullptr : table, seq * p.dense_slots, nullptr, 0, kvh, sb, se, g, r, qf,
+                    score_scale, st);
+        }
       }
       K::merge_row_groups(st);
       if (g == 0) {
@@ -656,7 +697,8 @@ __global__ __launch_bounds__(512) void paged_decode_stream_kernel(const PagedPar
 constexpr int kMergeThreads = 512;
 constexpr int kMergeBatch = 8;
 
-template <typename TQ, int D, int kMergeGroups>
+// kWindow: also the zeros of a decode row that has no key at all (nobody else writes it).
+template <typename TQ, int D, int kMergeGroups, bool kWindow>
 __global__ __launch_bounds__(kMergeThreads) void paged_decode_stream_merge_kernel(
     const PagedParams p, int wgs_i) {
   constexpr int kMergeCols = kMergeThreads / kMergeGroups;
@@ -668,7 +710,17 @@ __global__ __launch_bounds__(kMergeThreads) void paged_decode_stream_merge_kerne
   const int total = dense ? p.num_seqs * p.dense_keys : p.seq_prefix[p.num_seqs];
   const int begin = dense ? seq * p.dense_keys : p.seq_prefix[seq];
   const int end = dense ? begin + p.dense_keys : p.seq_prefix[seq + 1];
-  if (end == begin) return;  // whole workgroup: no barrier follows for it
+  if (end == begin) {  // whole workgroup: no barrier follows for it
+    if constexpr (kWindow) {
+      const int j0 = blockIdx.y * kMergeCols + threadIdx.x;
+      if (threadIdx.x < kMergeCols && j0 < p.hq * D / 4 && p.seq_lens[seq] == 1) {
+        const int64_t at = static_cast<int64_t>(p.cu_seqlens_q[seq]) * p.hq * D + 4 * j0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) Elem<TQ>::store(p.out, at + k, 0.0f);
+      }
+    }
+    return;
+  }
   const DecodeShares shares(total, wgs_i, p.stream_min_keys);
   const int first = shares.owner(begin);
   const int last = shares.owner(end - 1);
@@ -738,13 +790,28 @@ __global__ __launch_bounds__(kMergeThreads) void paged_decode_stream_merge_kerne
 
 // -------------------------------------------------------------- grid schedule
 
-template <typename TQ, typename TKV, int D, int GC>
+// kWindow: a row's keys are the entries of its windowed list, page ids read from the table; a
+// row without a key gets its zeros here.
+template <typename TQ, typename TKV, int D, int GC, bool kWindow>
 __global__ __launch_bounds__(512) void paged_decode_grid_kernel(const PagedParams p) {
   using K = Decode<TQ, TKV, D, GC>;
-  __shared__ int s_pages[kMaxSplitPages];
+  __shared__ int s_pages[kWindow ? 1 : kMaxSplitPages];
 
   int seq, row, visible;
-  if (!resolve_row(p, blockIdx.y, seq, row, visible)) return;
+  if constexpr (kWindow) {
+    if (!resolve_window_row(p, blockIdx.y, seq, row, visible)) return;
+    if (visible <= 0) {
+      if (blockIdx.x != 0 || blockIdx.z != 0) return;
+      for (int j = threadIdx.x; j < p.hq * D; j += blockDim.x) {
+        Elem<TQ>::store(p.out, static_cast<int64_t>(row) * p.hq * D + j, 0.0f);
+      }
+      return;
+    }
+  } else {
+    if (!resolve_row(p, blockIdx.y, seq, row, visible)) return;
+  }
+  const int all = visible;
+  if constexpr (kWindow) visible = window_keys(visible, p.window, p.sinks);
 
   const int nsplit = decode_num_splits(visible, p.split_tokens, p.max_splits);
   const int split = blockIdx.x;
@@ -762,11 +829,11 @@ __global__ __launch_bounds__(512) void paged_decode_grid_kernel(const PagedParam
   const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks;
   const int first_page = sb >> p.block_shift;
   const int n_pages = sb < se ? ((se - 1) >> p.block_shift) - first_page + 1 : 0;
-  const bool pages_in_lds = n_pages <= kMaxSplitPages;
+  const bool pages_in_lds = !kWindow && n_pages <= kMaxSplitPages;
   if (pages_in_lds) {
     for (int i = threadIdx.x; i < n_pages; i += blockDim.x) s_pages[i] = table[first_page + i];
   }
-  __syncthreads();
+  if constexpr (!kWindow) __syncthreads();
 
   int kvh, h0;
   if (!wave_unit<GC>(p, blockIdx.z * (blockDim.x / kWave) + wave, kvh, h0)) return;
@@ -775,8 +842,13 @@ __global__ __launch_bounds__(512) void paged_decode_grid_kernel(const PagedParam
   K::load_queries(p, row, h0, r, qf);
   typename K::State st;
   K::init(st);
-  K::stream(p, table, 0, pages_in_lds ? s_pages : nullptr, first_page, kvh, sb, se, g, r, qf,
-            p.scale * kLog2e, st);
+  if constexpr (kWindow) {
+    const WindowKeys keys{p.sinks, all - visible};
+    K::stream_window(p, table, keys, kvh, sb, se, g, r, qf, p.scale * kLog2e, st);
+  } else {
+    K::stream(p, table, 0, pages_in_lds ? s_pages : nullptr, first_page, kvh, sb, se, g, r, qf,
+              p.scale * kLog2e, st);
+  }
   K::merge_row_groups(st);
   if (g != 0) return;
   if (nsplit == 1) {
@@ -789,7 +861,7 @@ __global__ __launch_bounds__(512) void paged_decode_grid_kernel(const PagedParam
 
 // Combine the split partials of every (row, query head) that was split:
 // out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. One wave per (row, head).
-template <typename TQ, int D>
+template <typename TQ, int D, bool kWindow>
 __global__ __launch_bounds__(256) void paged_decode_grid_merge_kernel(const PagedParams p) {
   constexpr int kPerLane = (D + kWave - 1) / kWave;
   const int wave = threadIdx.x / kWave;
@@ -798,7 +870,12 @@ __global__ __launch_bounds__(256) void paged_decode_grid_merge_kernel(const Page
   if (head >= p.hq) return;
 
   int seq, row, visible;
-  if (!resolve_row(p, blockIdx.y, seq, row, visible)) return;
+  if constexpr (kWindow) {
+    if (!resolve_window_row(p, blockIdx.y, seq, row, visible) || visible <= 0) return;
+    visible = window_keys(visible, p.window, p.sinks);
+  } else {
+    if (!resolve_row(p, blockIdx.y, seq, row, visible)) return;
+  }
   const int nsplit = decode_num_splits(visible, p.split_tokens, p.max_splits);
   if (nsplit == 1) return;  // the decode kernel stored this row directly
 
@@ -854,7 +931,7 @@ int decode_waves(const PagedParams& p, int gc) {
 // 17.4 us a call, 8 of 300-2300 keys level, 16 of 1024 (16 pieces) 19.1 -> 20.0.
 constexpr int kWideMergePieces = 32;
 
-template <typename TQ, int D>
+template <typename TQ, int D, bool kWindow>
 hipError_t launch_stream_merge(const PagedParams& p, hipStream_t stream) {
   const int n4 = p.hq * D / 4;
   auto grid = [&](int groups) {
@@ -862,43 +939,47 @@ hipError_t launch_stream_merge(const PagedParams& p, hipStream_t stream) {
     return dim3(p.num_seqs, (n4 + cols - 1) / cols);
   };
   if (p.stream_wgs >= kWideMergePieces * p.num_seqs) {
-    paged_decode_stream_merge_kernel<TQ, D, 16><<<grid(16), kMergeThreads, 0, stream>>>(p, p.stream_wgs);
+    paged_decode_stream_merge_kernel<TQ, D, 16, kWindow><<<grid(16), kMergeThreads, 0, stream>>>(p, p.stream_wgs);
   } else {
-    paged_decode_stream_merge_kernel<TQ, D, 4><<<grid(4), kMergeThreads, 0, stream>>>(p, p.stream_wgs);
+    paged_decode_stream_merge_kernel<TQ, D, 4, kWindow><<<grid(4), kMergeThreads, 0, stream>>>(p, p.stream_wgs);
   }
   return hipGetLastError();
 }
 
-template <typename TQ, typename TKV, int D, int GC>
+template <typename TQ, typename TKV, int D, int GC, bool kWindow>
 hipError_t launch_decode_g(const PagedParams& p, hipStream_t stream) {
   const int units = p.hk * (p.hq / p.hk / GC);
   const int waves = decode_waves(p, GC);
   constexpr int kHeadsPerMergeBlock = 4;
   if (p.stream_wgs > 0) {
     if (units > 8) return hipErrorInvalidValue;  // planner keeps stream mode to <= 8 units
-    paged_decode_stream_kernel<TQ, TKV, D, GC, false>
+    paged_decode_stream_kernel<TQ, TKV, D, GC, false, kWindow>
         <<<p.stream_wgs, waves * kWave, 0, stream>>>(p, FreshParams{});
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    return launch_stream_merge<TQ, D>(p, stream);
+    return launch_stream_merge<TQ, D, kWindow>(p, stream);
   }
   const dim3 grid(p.max_splits, p.by_row ? p.num_tokens : p.num_seqs, (units + waves - 1) / waves);
-  paged_decode_grid_kernel<TQ, TKV, D, GC><<<grid, waves * kWave, 0, stream>>>(p);
+  paged_decode_grid_kernel<TQ, TKV, D, GC, kWindow><<<grid, waves * kWave, 0, stream>>>(p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.max_splits == 1) return err;
   const dim3 mgrid((p.hq + kHeadsPerMergeBlock - 1) / kHeadsPerMergeBlock,
                    p.by_row ? p.num_tokens : p.num_seqs);
-  paged_decode_grid_merge_kernel<TQ, D><<<mgrid, kHeadsPerMergeBlock * kWave, 0, stream>>>(p);
+  paged_decode_grid_merge_kernel<TQ, D, kWindow><<<mgrid, kHeadsPerMergeBlock * kWave, 0, stream>>>(p);
   return hipGetLastError();
 }
 
 template <typename TQ, typename TKV, int D>
 hipError_t launch_decode_d(const PagedParams& p, hipStream_t stream) {
-  switch (decode_group_chunk(p.hq / p.hk)) {
-    case 4: return launch_decode_g<TQ, TKV, D, 4>(p, stream);
-    case 2: return launch_decode_g<TQ, TKV, D, 2>(p, stream);
-    default: return launch_decode_g<TQ, TKV, D, 1>(p, stream);
+  const int gc = decode_group_chunk(p.hq / p.hk);
+  if (p.window > 0) {
+    if (gc == 4) return launch_decode_g<TQ, TKV, D, 4, true>(p, stream);
+    return gc == 2 ? launch_decode_g<TQ, TKV, D, 2, true>(p, stream)
+                   : launch_decode_g<TQ, TKV, D, 1, true>(p, stream);
   }
+  if (gc == 4) return launch_decode_g<TQ, TKV, D, 4, false>(p, stream);
+  return gc == 2 ? launch_decode_g<TQ, TKV, D, 2, false>(p, stream)
+                 : launch_decode_g<TQ, TKV, D, 1, false>(p, stream);
 }
 
 template <typename TQ, typename TKV>
@@ -921,11 +1002,11 @@ hipError_t launch_fresh_g(const PagedParams& p, const FreshParams& f, hipStream_
   constexpr int D = 128;
   const int units = p.hk * (p.hq / p.hk / GC);
   if (units > 8) return hipErrorInvalidValue;  // planner keeps stream mode to <= 8 units
-  paged_decode_stream_kernel<T, T, D, GC, true>
+  paged_decode_stream_kernel<T, T, D, GC, true, false>
       <<<p.stream_wgs, decode_waves(p, GC) * kWave, 0, stream>>>(p, f);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  return launch_stream_merge<T, D>(p, stream);
+  return launch_stream_merge<T, D, false>(p, stream);
 }
 
 template <typename T>

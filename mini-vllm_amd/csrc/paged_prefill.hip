@@ -163,6 +163,28 @@ struct Cursor {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// The key list of an item whose first query stands at position p0 (paged_attention.hpp): entry v
+// at position v for v < front, v + gap from there on, front a multiple of `align`. [hole, seen) are
+// the entries that no query of the item sees: none with align 1; with align a run of `align`
+// keys always holds a key that is seen, so the page of such a run is the sequence's own still.
+struct WindowList {
+  int front, gap, hole, seen;
+};
+template <int align>
+__device__ __forceinline__ WindowList window_list(const PagedParams& p, int p0) {
+  WindowList w;
+  const int lo = max(p0 - p.window + 1, 0);  // the first key of the first query's window
+  w.front = min(p.sinks, lo);
+  w.front = (w.front + align - 1) / align * align;
+  w.gap = max(lo / align * align - w.front, 0);
+  w.seen = lo - w.gap;
+  w.hole = min(p.sinks, w.seen);
+  return w;
+}
+__device__ __forceinline__ int list_position(const WindowList& w, int v) {
+  return v < w.front ? v : v + w.gap;
+}
+
 // Share index of workgroup `bid` of `n`: workgroups are dispatched to the XCDs round
 // robin, so this gives the workgroups of one XCD consecutive shares (the items one L2
 // serves are few, their K/V tiles reused from it).
@@ -294,8 +316,12 @@ struct PairPiece {
 };
 
 // Key tiles walked by an item of `qt` query positions.
-__device__ __forceinline__ int pair_item_tiles(int context, int len, int q, int qt) {
-  return (context - len + min((q + 1) * qt, len) + kTileKeys - 1) / kTileKeys;
+constexpr int kPairAlign = 16;  // a wave's keys of a tile lie in one page (of >= 16 keys)
+template <bool kWindow>
+__device__ __forceinline__ int pair_item_tiles(const PagedParams& p, int context, int len, int q, int qt) {
+  int end = context - len + min((q + 1) * qt, len);
+  if constexpr (kWindow) end -= window_list<kPairAlign>(p, context - len + q * qt).gap;
+  return (end + kTileKeys - 1) / kTileKeys;
 }
 
 // Query tiles of a sequence (a decode row has none here).
@@ -331,23 +357,23 @@ __device__ __forceinline__ bool pair_fits(const PagedParams& p, int cols, int ra
 }
 
 // Pieces (low half) and cut items' slots (high half; both below 2^15) of a sequence.
-template <int QT>
+template <int QT, bool kWindow>
 __device__ __forceinline__ int pair_count(const PagedParams& p, int ctx, int len, int length) {
   const int qts = pair_query_tiles(len, QT);
   int both = 0;
   for (int q = 0; q < qts; ++q) {
-    const int pcs = pair_pieces(p, pair_item_tiles(ctx, len, q, QT), length);
+    const int pcs = pair_pieces(p, pair_item_tiles<kWindow>(p, ctx, len, q, QT), length);
     both += pcs | (pcs > 1 ? pcs << 16 : 0);
   }
   return both;
 }
 
 // The `r`th piece of a sequence, whose cut items' slots start at out.slot0.
-template <int QT>
+template <int QT, bool kWindow>
 __device__ __forceinline__ void pair_locate(const PagedParams& p, int ctx, int len, int length, int r,
                                             PairPiece& out) {
   for (out.q = 0;; ++out.q) {
-    const int nt = pair_item_tiles(ctx, len, out.q, QT);
+    const int nt = pair_item_tiles<kWindow>(p, ctx, len, out.q, QT);
     out.pieces = pair_pieces(p, nt, length);
     if (r < out.pieces) {
       out.piece = r;
@@ -365,7 +391,7 @@ __device__ __forceinline__ void pair_locate(const PagedParams& p, int ctx, int l
 // data, no launch before, no barrier). The positions past the last piece end here; they come
 // last, so that the pieces are dealt to empty CUs one each (first, they left some CUs two
 // pieces and others none: a 512-token chunk after 8000 keys 60 us against 57).
-template <int QT, bool kFp8>
+template <int QT, bool kFp8, bool kWindow>
 __device__ __forceinline__ bool pair_piece(const PagedParams& p, int cols, int rank, PairPiece& out) {
   const int lane = threadIdx.x % kWave;
   const int len = lane < p.num_seqs ? p.seq_lens[lane] : 0;
@@ -401,32 +427,32 @@ __device__ __forceinline__ bool pair_piece(const PagedParams& p, int cols, int r
     out.q = __builtin_amdgcn_readlane(qts, out.s) - 1 - q_from_last;
     out.piece = out.tb = out.slot0 = 0;
     out.pieces = 1;
-    out.te = pair_item_tiles(__builtin_amdgcn_readlane(ctx, out.s), __builtin_amdgcn_readlane(len, out.s),
-                             out.q, QT);
+    out.te = pair_item_tiles<kWindow>(p, __builtin_amdgcn_readlane(ctx, out.s),
+                                      __builtin_amdgcn_readlane(len, out.s), out.q, QT);
     return true;
   }
   int length = 0;
   {
     int tiles = 0;
-    for (int q = 0; q < qts; ++q) tiles += pair_item_tiles(ctx, len, q, QT);
+    for (int q = 0; q < qts; ++q) tiles += pair_item_tiles<kWindow>(p, ctx, len, q, QT);
     const int items = wave_total(qts), total = wave_total(tiles);
-    const int own = qts > 0 ? pair_item_tiles(ctx, len, qts - 1, QT) : 0;
+    const int own = qts > 0 ? pair_item_tiles<kWindow>(p, ctx, len, qts - 1, QT) : 0;
     const int longest = static_cast<int>(wave_max(static_cast<float>(own)));  // (below 2^24)
     const bool whole = pair_stays_whole<QT, kFp8>(p, cols, total, longest);
     length = whole ? max(longest, 1) : pair_piece_tiles(p, cols, total);
     for (int i = 0; i < 12 && !whole; ++i) {
-      if (pair_fits(p, cols, wave_total(pair_count<QT>(p, ctx, len, length) & 0xffff), items)) break;
+      if (pair_fits(p, cols, wave_total(pair_count<QT, kWindow>(p, ctx, len, length) & 0xffff), items)) break;
       length += (length + 15) / 16;
     }
   }
-  const int both = pair_count<QT>(p, ctx, len, length);
+  const int both = pair_count<QT, kWindow>(p, ctx, len, length);
   const int before = wave_inclusive_scan(both) - both;
   const int first = before & 0xffff;
   const uint64_t mine = __builtin_amdgcn_ballot_w64(rank >= first && rank < first + (both & 0xffff));
   if (mine == 0) return false;
   out.s = __builtin_ctzll(mine);
   out.slot0 = __builtin_amdgcn_readlane(before, out.s) >> 16;
-  pair_locate<QT>(p, __builtin_amdgcn_readlane(ctx, out.s), __builtin_amdgcn_readlane(len, out.s), length,
+  pair_locate<QT, kWindow>(p, __builtin_amdgcn_readlane(ctx, out.s), __builtin_amdgcn_readlane(len, out.s), length,
                   rank - (__builtin_amdgcn_readlane(before, out.s) & 0xffff), out);
   // (the bounds above rule this out; a slot is never written past the workspace)
   return out.pieces == 1 || out.slot0 + out.pieces <= p.pf_slots;
@@ -442,7 +468,7 @@ __device__ __forceinline__ void pair_store(const PagedParams& p, int rank, const
 // listed in LDS, then held a lane each, 64 at a time. (Every workgroup scanning all sequences
 // for itself, once per length tried, took longer than the prefill: one 512-token chunk after
 // 7000 keys among 500 decodes 309 us a call, so 275.)
-template <int QT, bool kFp8>
+template <int QT, bool kFp8, bool kWindow>
 __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const PagedParams p) {
   constexpr int kAhead = 8;
   __shared__ int s_seq[kMaxStreamSeqs], s_len[kMaxStreamSeqs], s_ctx[kMaxStreamSeqs];
@@ -484,8 +510,8 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
     take(base);
     const int qts = pair_query_tiles(len, QT);
     int tiles = 0;
-    for (int q = 0; q < qts; ++q) tiles += pair_item_tiles(ctx, len, q, QT);
-    const int own = qts > 0 ? pair_item_tiles(ctx, len, qts - 1, QT) : 0;
+    for (int q = 0; q < qts; ++q) tiles += pair_item_tiles<kWindow>(p, ctx, len, q, QT);
+    const int own = qts > 0 ? pair_item_tiles<kWindow>(p, ctx, len, qts - 1, QT) : 0;
     total += wave_total(tiles);
     items += wave_total(qts);
     longest = max(longest, static_cast<int>(wave_max(static_cast<float>(own))));  // (below 2^24)
@@ -496,7 +522,7 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
     int ranks = 0;
     for (int base = 0; base < chunks; base += kWave) {
       if (chunks > kWave) take(base);
-      ranks += wave_total(pair_count<QT>(p, ctx, len, length) & 0xffff);
+      ranks += wave_total(pair_count<QT, kWindow>(p, ctx, len, length) & 0xffff);
     }
     if (pair_fits(p, cols, ranks, items)) break;
     length += (length + 15) / 16;
@@ -504,7 +530,7 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
   int ranks = 0, slots = 0;
   for (int base = 0; base < chunks; base += kWave) {
     if (chunks > kWave) take(base);
-    const int both = pair_count<QT>(p, ctx, len, length);
+    const int both = pair_count<QT, kWindow>(p, ctx, len, length);
     const int incl = wave_inclusive_scan(both);
     const int all = __builtin_amdgcn_readlane(incl, kWave - 1);
     int rank = ranks + ((incl - both) & 0xffff), slot0 = slots + ((incl - both) >> 16);
@@ -512,7 +538,7 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
     PairPiece w{};
     w.s = base + lane < chunks ? s_seq[base + lane] : 0;
     for (w.q = 0; w.q < qts; ++w.q) {
-      const int nt = pair_item_tiles(ctx, len, w.q, QT);
+      const int nt = pair_item_tiles<kWindow>(p, ctx, len, w.q, QT);
       w.pieces = pair_pieces(p, nt, length);
       w.slot0 = slot0;
       if (w.pieces > 1) slot0 += w.pieces;
@@ -531,7 +557,9 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
 
 }  // namespace
 
-template <typename TQ, typename TKV, int D, int HCW, int HS>
+// kWindow (on the grid only: windowed items are of about one length): an item's keys are the
+// entries of its windowed list, which with no alignment to keep holds no entry that nobody sees.
+template <typename TQ, typename TKV, int D, int HCW, int HS, bool kWindow>
 __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedParams p) {
   constexpr int kThreads = 256 * HS;
   constexpr int HW = HCW * HS;                  // query heads per work item
@@ -551,7 +579,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
 
   __shared__ __align__(16) uint16_t k_lds[2][kTileKeys * kKStride];
   __shared__ __align__(16) uint16_t v_lds[2][D * kVStride];
-  __shared__ int s_prefix[kMaxStreamSeqs + 1];
+  __shared__ int s_prefix[kWindow ? 1 : kMaxStreamSeqs + 1];
 
   const int tid = threadIdx.x;
   const int wave = uniform(tid / kWave);
@@ -565,13 +593,22 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
   const int group = p.hq / p.hk;
   const int chunks = group / HW;
   const int cols = p.hk * chunks;
-  const bool stream = p.pf_wgs > 0;
+  const bool stream = !kWindow && p.pf_wgs > 0;
   int share = xcd_share(blockIdx.x, gridDim.x);
 
   // ---- this workgroup's units [u0, u1) and the cursor at u0.
   Cursor cur;
   int u0, u1;
-  if (!prefill_work<kThreads>(p, cols, share, s_prefix, cur, u0, u1)) return;
+  if (!prefill_work<kThreads, kWindow>(p, cols, share, s_prefix, cur, u0, u1)) return;
+  // Positions below are entries of the item's key list (itself, but for kWindow).
+  WindowList list{};
+  if constexpr (kWindow) {
+    list = window_list<1>(p, cur.context - cur.len + cur.q * kPrefillQueryTile);
+    cur.context -= list.gap;
+    cur.nt = u1 = prefill_item_tiles(cur.context, cur.len, cur.q);
+    if (u1 <= 0) return;
+  }
+  auto position = [&](int v) __attribute__((always_inline)) { return kWindow ? list_position(list, v) : v; };
   auto advance = [&](Cursor& k) __attribute__((always_inline)) {
     ++k.u;
     if (++k.t < k.nt) return;
@@ -613,12 +650,12 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     const int last = k.context - 1;
     const int kvh = k.c / chunks;  // fp8 scales only
 #pragma unroll
-    for (int u = 0; u < kKUnits; ++u) kpg[S][u] = table[min(key0 + k_key(u), last) >> p.block_shift];
+    for (int u = 0; u < kKUnits; ++u) kpg[S][u] = table[position(min(key0 + k_key(u), last)) >> p.block_shift];
 #pragma unroll
     for (int u = 0; u < kVUnits; ++u) {
 #pragma unroll
       for (int j = 0; j < kVKeys; ++j) {
-        vpg[S][u][j] = table[min(key0 + kVKeys * v_grp(u) + j, last) >> p.block_shift];
+        vpg[S][u][j] = table[position(min(key0 + kVKeys * v_grp(u) + j, last)) >> p.block_shift];
       }
     }
     if constexpr (kFp8) {
@@ -648,7 +685,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     const uint32_t head_off = static_cast<uint32_t>((k.c / chunks) * p.kv_head_bytes);
 #pragma unroll
     for (int u = 0; u < kKUnits; ++u) {
-      const int key = min(key0 + k_key(u), last);
+      const int key = position(min(key0 + k_key(u), last));
       const uint64_t off = pool_offset(kpg[S][u], key, head_off + k_dim(u) * kElemBytes);
       kreg[S][u] = Stage<TQ, TKV>::load(kpool + off, kFp8 ? ksc[S][u] : 1.0f);
     }
@@ -656,7 +693,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     for (int u = 0; u < kVUnits; ++u) {
 #pragma unroll
       for (int j = 0; j < kVKeys; ++j) {
-        const int key = min(key0 + kVKeys * v_grp(u) + j, last);
+        const int key = position(min(key0 + kVKeys * v_grp(u) + j, last));
         const uint64_t off = pool_offset(vpg[S][u][j], key, head_off + v_dim(u) * kElemBytes);
         vreg[S][u][j] = Stage<TQ, TKV>::load(vpool + off, kFp8 ? vsc[S][u][j] : 1.0f);
       }
@@ -751,7 +788,24 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     }
 
     // Causal mask, on tiles crossing the diagonal only: score (kb, r) of this lane is
-    // key key0 + 4*hsel + (32kb + 8(r/4) + r%4); visible while below my_visible.
+    // key key0 + 4*hsel + (32kb + 8(r/4) + r%4); visible while below my_visible. And the
+    // window's, on tiles that hold keys between the sinks and a query's own first one.
+    if constexpr (kWindow) {
+      if (key0 < w_kv_end - p.window && key0 + kTileKeys > p.sinks) {
+        const int lo = my_visible - p.window - key0 - 4 * hsel, front = p.sinks - key0 - 4 * hsel;
+#pragma unroll
+        for (int h = 0; h < HCW; ++h) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int e = kb * 32 + 8 * (r >> 2) + (r & 3);
+              if (e >= front && e < lo) s[h][kb][r] = -INFINITY;
+            }
+          }
+        }
+      }
+    }
     if (key0 + kTileKeys > w_kv_full) {
       asm volatile("" ::: "memory");  // keep this a branch: most tiles need no mask
       const int lim = my_valid ? my_visible - key0 - 4 * hsel : INT_MIN;
@@ -1360,7 +1414,14 @@ __global__ __launch_bounds__(256) void paged_prefill_lds_kernel(const PagedParam
 //    scale, into the same buffers before the barrier. With eight waves a tile is converted for
 //    twice the positions: five chunks of 61-512 tokens beside 28 decodes 93 -> 80 us a call,
 //    with the schedule's balance.
-template <typename TQ, typename TKV, int kWaves, bool kSplit>
+//
+// kWindow: an item's tiles are those of its windowed key list (WindowList): the sinks' 16-key
+// runs, then the runs from the first query's window on, so what an item walks goes by the window
+// and not by the context. A tile's staging adds the gap to its position (a scalar add); rows that
+// no query of the item sees are staged as a seen row of their page, so nothing behind the window
+// is used, whatever it holds; a query's own window is a second comparison per score, on the one
+// or two tiles that hold a window's edge.
+template <typename TQ, typename TKV, int kWaves, bool kSplit, bool kWindow>
 __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(const PagedParams p) {
   constexpr bool kFp8 = std::is_same_v<TKV, fp8_t>;
   constexpr int D = 128;
@@ -1414,7 +1475,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
       if (a.w == 0) return;
       piece = PairPiece{a.x, a.y, a.z, a.w, b.x, b.y, b.z};
     } else {
-      const bool got = pair_piece<QT, kFp8>(p, cols, rank, piece);
+      const bool got = pair_piece<QT, kFp8, kWindow>(p, cols, rank, piece);
       if (p.pf_pieces > 1 && c == 0 && tid == 0) {  // what the merge needs to know
         pair_store(p, rank, got ? piece : PairPiece{});
       }
@@ -1432,13 +1493,21 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
     c = blockIdx.x;
   }
   const int len = sload(p.seq_lens + s);
-  const int context = sload(p.context_lens + s);
+  const int held = sload(p.context_lens + s);
   if constexpr (!kSplit) {
     if (len <= 1) return;  // a decode row: the decode kernel has it
     if (qt * QT >= len) return;
     tb = 0;
-    te = pair_item_tiles(context, len, qt, QT);
+    te = pair_item_tiles<kWindow>(p, held, len, qt, QT);
+    if (kWindow && te <= 0) return;
   }
+  // Positions below are entries of the item's key list (itself, but for kWindow).
+  WindowList list{};
+  if constexpr (kWindow) {
+    list = window_list<kPairAlign>(p, held - len + qt * QT);
+    list = WindowList{uniform(list.front), uniform(list.gap), uniform(list.hole), uniform(list.seen)};
+  }
+  const int context = held - list.gap;
   const int kvh = c / chunks;
 
   const float score_c = p.scale * kLog2e;  // > 0 (the dispatcher's condition)
@@ -1459,6 +1528,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
   const int my_local = w_first + l32;
   const bool my_valid = my_local < len;
   const int my_visible = offset + my_local + 1;
+  const int my_lo = kWindow ? my_visible - p.window : 0;             // first entry of its window
+  const int w_lo_last = kWindow ? w_kv_end - p.window : 0;           // of its last query's
   const int row_base = sload(p.cu_seqlens_q + s);
   const int head0 = kvh * group + (c % chunks) * 2 + hs;
 
@@ -1502,7 +1573,9 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
   float ks_lane = 0.0f, vs_lane = 0.0f;
   auto take_pages = [&](int t) __attribute__((always_inline)) {  // of the block holding tile t
     const int tile = min((t & -kWave) + lane, te - 1);
-    pages = load_dword_now(table + (min(tile * kTileKeys + KW * wave, context - 1) >> p.block_shift));
+    int at = min(tile * kTileKeys + KW * wave, context - 1);
+    if constexpr (kWindow) at = list_position(list, at);
+    pages = load_dword_now(table + (at >> p.block_shift));
     if constexpr (kFp8) {
       const int64_t si = static_cast<int64_t>(pages) * p.hk + kvh;
       ks_lane = __int_as_float(load_dword_now(p.k_scales + si));
@@ -1522,15 +1595,23 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
     const int key0 = t * kTileKeys + KW * wave;
     const int last = context - 1;
     const uint64_t head = static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_bytes + head_off;
-    if (key0 + KW - 1 <= last) {
-      const uint64_t base = head + static_cast<uint32_t>(key0 & p.block_mask) * row_bytes;
+    const bool seen = !kWindow || key0 >= list.seen || key0 + KW <= list.hole;
+    if (key0 + KW - 1 <= last && seen) {
+      const int at = kWindow ? uniform(list_position(list, key0)) : key0;
+      const uint64_t base = head + static_cast<uint32_t>(at & p.block_mask) * row_bytes;
 #pragma unroll
       for (int j = 0; j < kCopies; ++j) copy_to_lds(pool + base, src_off[j], dst + 1024 * j);
     } else {
 #pragma unroll
       for (int j = 0; j < kCopies; ++j) {
-        const uint32_t row = static_cast<uint32_t>(min(key0 + kKeysPerCopy * j + lane / kRowLanes, last) &
-                                                   p.block_mask) * row_bytes;
+        int at = min(key0 + kKeysPerCopy * j + lane / kRowLanes, last);
+        if constexpr (kWindow) {
+          // (a run of 16 that starts before the hole holds its entry hole - 1, one that does not
+          // its entry `seen`)
+          if (at >= list.hole && at < list.seen) at = (at & -kPairAlign) < list.hole ? list.hole - 1 : list.seen;
+          at = list_position(list, at);
+        }
+        const uint32_t row = static_cast<uint32_t>(at & p.block_mask) * row_bytes;
         copy_to_lds(pool + head, row + chunk_of(j), dst + 1024 * j);
       }
     }
@@ -1611,6 +1692,20 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
   };
   auto mask = [&](int t, f32x16 (&sc)[2]) __attribute__((always_inline)) {
     const int key0 = t * kTileKeys;
+    if constexpr (kWindow) {
+      // The window's edge: entries from the sinks up to the query's own first key.
+      if (key0 < w_lo_last && key0 + kTileKeys > p.sinks) {
+        const int lo = my_lo - key0 - 4 * hsel, front = p.sinks - key0 - 4 * hsel;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int e = kb * 32 + 8 * (r >> 2) + (r & 3);
+            if (e >= front && e < lo) sc[kb][r] = -INFINITY;
+          }
+        }
+      }
+    }
     if (key0 + kTileKeys > w_kv_full) {
       const int lim = my_valid ? my_visible - key0 - 4 * hsel : INT_MIN;
 #pragma unroll
@@ -2069,50 +2164,50 @@ __global__ __launch_bounds__(kMergeThreads) void paged_prefill_merge_kernel(cons
 
 namespace {
 
-template <typename TQ, typename TKV, int D, int HCW, int HS>
+template <typename TQ, typename TKV, int D, int HCW, int HS, bool kWindow>
 void launch_prefill_cfg(const PagedParams& p, int max_query_len, hipStream_t stream) {
   constexpr int HW = HCW * HS;
-  if (p.pf_wgs > 0) {
-    paged_prefill_kernel<TQ, TKV, D, HCW, HS><<<p.pf_wgs, 256 * HS, 0, stream>>>(p);
+  if (!kWindow && p.pf_wgs > 0) {
+    paged_prefill_kernel<TQ, TKV, D, HCW, HS, false><<<p.pf_wgs, 256 * HS, 0, stream>>>(p);
     paged_prefill_merge_kernel<TQ, D, HW><<<kMergeSub * p.pf_wgs, kMergeThreads, 0, stream>>>(p);
   } else {
     const int cols = p.hk * (p.hq / p.hk / HW);
     const int qtiles = (max_query_len + kPrefillQueryTile - 1) / kPrefillQueryTile;
     const dim3 grid(cols, p.num_seqs, qtiles);
-    paged_prefill_kernel<TQ, TKV, D, HCW, HS><<<grid, 256 * HS, 0, stream>>>(p);
+    paged_prefill_kernel<TQ, TKV, D, HCW, HS, kWindow><<<grid, 256 * HS, 0, stream>>>(p);
   }
 }
 
 // The pair kernel by its schedule (pf_pieces >= 1: a workgroup per position of it; pieces
 // merged after) or on the item grid.
-template <typename TQ, typename TKV, int kWaves>
+template <typename TQ, typename TKV, int kWaves, bool kWindow>
 void launch_prefill_ranked(const PagedParams& p, hipStream_t stream) {
   constexpr int QT = kWaves * 16;
   const int grid = p.hq / 2 * p.pf_ranks;
   if (p.num_seqs > kWave) {
-    paged_prefill_schedule_kernel<QT, std::is_same_v<TKV, fp8_t>><<<1, kWave, 0, stream>>>(p);
+    paged_prefill_schedule_kernel<QT, std::is_same_v<TKV, fp8_t>, kWindow><<<1, kWave, 0, stream>>>(p);
   }
-  paged_prefill_pair_kernel<TQ, TKV, kWaves, true><<<grid, kWaves * kWave, 0, stream>>>(p);
+  paged_prefill_pair_kernel<TQ, TKV, kWaves, true, kWindow><<<grid, kWaves * kWave, 0, stream>>>(p);
   if (p.pf_pieces > 1) {
     paged_prefill_pair_merge_kernel<TQ, QT><<<grid, kPairMergeThreads, 0, stream>>>(p);
   }
 }
 
-template <typename TQ, typename TKV>
+template <typename TQ, typename TKV, bool kWindow>
 void launch_prefill_pair(const PagedParams& p, int max_query_len, hipStream_t stream) {
   const int cols = p.hq / 2;
   if (p.pf_pieces >= 1) {
-    if (p.pf_tile == 128) launch_prefill_ranked<TQ, TKV, 8>(p, stream);
-    else launch_prefill_ranked<TQ, TKV, 4>(p, stream);
+    if (p.pf_tile == 128) launch_prefill_ranked<TQ, TKV, 8, kWindow>(p, stream);
+    else launch_prefill_ranked<TQ, TKV, 4, kWindow>(p, stream);
     return;
   }
   if (p.pf_tile == 128) {
     const int wide = (max_query_len + 127) / 128;
-    paged_prefill_pair_kernel<TQ, TKV, 8, false><<<dim3(cols, p.num_seqs, wide), 512, 0, stream>>>(p);
+    paged_prefill_pair_kernel<TQ, TKV, 8, false, kWindow><<<dim3(cols, p.num_seqs, wide), 512, 0, stream>>>(p);
     return;
   }
   const int qtiles = (max_query_len + 63) / 64;
-  paged_prefill_pair_kernel<TQ, TKV, 4, false><<<dim3(cols, p.num_seqs, qtiles), 256, 0, stream>>>(p);
+  paged_prefill_pair_kernel<TQ, TKV, 4, false, kWindow><<<dim3(cols, p.num_seqs, qtiles), 256, 0, stream>>>(p);
 }
 
 template <typename TQ>
@@ -2134,22 +2229,28 @@ hipError_t launch_prefill_d(const PagedParams& p, int max_query_len, hipStream_t
   if constexpr (D == 128) {
     if (p.block_shift >= 4 && p.scale > 0.0f && !p.pf_register_staging) {
       if (prefill_item_heads(p.hq / p.hk) == 2) {
-        launch_prefill_pair<TQ, TKV>(p, max_query_len, stream);
+        if (p.window > 0) launch_prefill_pair<TQ, TKV, true>(p, max_query_len, stream);
+        else launch_prefill_pair<TQ, TKV, false>(p, max_query_len, stream);
         return hipGetLastError();
       }
       if constexpr (std::is_same_v<TQ, TKV>) {
-        launch_prefill_lds<TQ>(p, max_query_len, stream);
-        return hipGetLastError();
+        if (p.window == 0) {
+          launch_prefill_lds<TQ>(p, max_query_len, stream);
+          return hipGetLastError();
+        }
       }
     }
   }
   // Both heads of an even GQA group in one wave (HCW = 2) would share K/V fragments,
   // but needs ~450 registers: one wave per SIMD and no softmax/MFMA overlap. Measured
   // at config 3 it ran 25-40% slower than a wave per head, two waves per SIMD.
-  if (prefill_item_heads(p.hq / p.hk) == 1) {
-    launch_prefill_cfg<TQ, TKV, D, 1, 1>(p, max_query_len, stream);
+  const bool one = prefill_item_heads(p.hq / p.hk) == 1;
+  if (p.window > 0) {
+    if (one) launch_prefill_cfg<TQ, TKV, D, 1, 1, true>(p, max_query_len, stream);
+    else launch_prefill_cfg<TQ, TKV, D, 1, 2, true>(p, max_query_len, stream);
   } else {
-    launch_prefill_cfg<TQ, TKV, D, 1, 2>(p, max_query_len, stream);
+    if (one) launch_prefill_cfg<TQ, TKV, D, 1, 1, false>(p, max_query_len, stream);
+    else launch_prefill_cfg<TQ, TKV, D, 1, 2, false>(p, max_query_len, stream);
   }
   return hipGetLastError();
 }

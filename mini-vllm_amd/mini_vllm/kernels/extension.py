@@ -32,6 +32,7 @@ import sys
 import sysconfig
 import threading
 from concurrent.futures import ThreadPoolExecutor
+from contextlib import nullcontext
 from pathlib import Path
 from typing import Any
 
@@ -360,6 +361,12 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.mvllm_paged_attention.argtypes = (
         [p] * 10 + [i32] * 6 + [i64, i32, i32, i32, f32, i32, i32, opts, p, u64, p]
     )
+    lib.mvllm_paged_window_attention_plan.restype = ctypes.c_int
+    lib.mvllm_paged_window_attention_plan.argtypes = [i32] * 12 + [opts, ctypes.POINTER(_Plan)]
+    lib.mvllm_paged_window_attention.restype = ctypes.c_int
+    lib.mvllm_paged_window_attention.argtypes = (
+        [p] * 10 + [i32] * 6 + [i64] + [i32] * 5 + [f32, i32, i32, opts, p, u64, p]
+    )
     lib.mvllm_paged_attention_noalloc.restype = ctypes.c_int
     lib.mvllm_paged_attention_noalloc.argtypes = (
         [p] * 10 + [i32] * 6 + [i64, i32, i32, i32, f32, i32, i32, opts, p]
@@ -435,6 +442,8 @@ EXPORTED_SYMBOLS = (
     "mvllm_paged_attention_plan",
     "mvllm_paged_attention",
     "mvllm_paged_attention_noalloc",
+    "mvllm_paged_window_attention_plan",
+    "mvllm_paged_window_attention",
     "mvllm_rmsnorm",
     "mvllm_rope",
     "mvllm_swiglu",
@@ -506,6 +515,14 @@ def _stream(device: torch.device) -> int:
     which an eager prefill iteration pays for every one of its ~400 launches."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _on_device(device: torch.device):
+    """A context in which ``device`` is the current one: a launch goes to the current device,
+    whatever device its stream is of."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
 
 
 class HipExtension:
@@ -1595,6 +1612,98 @@ class HipExtension:
                 _stream(q.device),
             )
         )
+        return out
+
+    def paged_window_attention_plan(
+        self,
+        num_tokens: int,
+        num_seqs: int,
+        num_q_heads: int,
+        num_kv_heads: int,
+        head_dim: int,
+        block_size: int,
+        max_query_len: int,
+        max_context_len: int,
+        window: int,
+        sinks: int,
+        q_dtype: torch.dtype,
+        kv_dtype: torch.dtype,
+        plan_options: dict[str, Any] | None = None,
+    ) -> dict[str, int]:
+        """The library's plan for a windowed call of these sizes
+        (``mvllm_paged_window_attention_plan``), as :meth:`paged_attention_plan`."""
+        plan = _Plan()
+        opts = make_plan_options(plan_options)
+        self._check(self.lib.mvllm_paged_window_attention_plan(
+            num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_query_len,
+            max_context_len, window, sinks, DTYPE_CODES.get(q_dtype, -1),
+            DTYPE_CODES.get(kv_dtype, -1), None if opts is None else ctypes.byref(opts),
+            ctypes.byref(plan)))
+        out = {name: getattr(plan, name) for name, _ in _Plan._fields_}
+        out["decode_mode"] = DECODE_MODES.get(out["decode_mode"], out["decode_mode"])
+        return out
+
+    def paged_window_attention(
+        self,
+        q: torch.Tensor,
+        key_pool: torch.Tensor,
+        value_pool: torch.Tensor,
+        block_tables: torch.Tensor,
+        cu_seqlens_q: torch.Tensor,
+        context_lens: torch.Tensor,
+        seq_lens: torch.Tensor,
+        max_query_len: int,
+        max_context_len: int,
+        window: int,
+        sinks: int,
+        scale: float,
+        k_scale: torch.Tensor | None = None,
+        v_scale: torch.Tensor | None = None,
+        out: torch.Tensor | None = None,
+        plan_options: dict[str, Any] | None = None,
+    ) -> torch.Tensor:
+        """:meth:`paged_attention` over a sliding window with sinks: a query at position p sees
+        the keys ``j <= p`` with ``j > p - window`` or ``j < sinks``. Pages that no query of the
+        call sees are not read (their table entries may be -1)."""
+        cu_seqlens_q, context_lens, seq_lens = self._paged_checks(
+            q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens, seq_lens,
+            max_query_len, max_context_len, k_scale, v_scale)
+        num_blocks, block_size, num_kv_heads, head_dim = key_pool.shape
+        if (key_pool.data_ptr() | value_pool.data_ptr()) % 16:
+            raise RuntimeError("paged_window_attention: the pools must be 16-byte aligned")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
+              or out.device != q.device or out.data_ptr() % 16):
+            raise RuntimeError("paged_window_attention: out must be a contiguous, 16-byte aligned "
+                               "tensor shaped like q on q's device")
+        num_tokens, num_q_heads, _ = q.shape
+        num_sequences = seq_lens.shape[0]
+        if num_tokens == 0 or num_sequences == 0:
+            return out
+        if q.data_ptr() % 16:
+            q = q.clone()
+        opts = make_plan_options(plan_options)
+        opts_ref = None if opts is None else ctypes.byref(opts)
+        # (an int beyond int32 is every key, as the largest int32 is)
+        window, sinks = (min(max(int(n), -1), 2**31 - 1) for n in (window, sinks))
+        sizes = (num_tokens, num_sequences, num_q_heads, num_kv_heads, head_dim, block_size)
+        codes = (DTYPE_CODES[q.dtype], DTYPE_CODES[key_pool.dtype])
+        plan = _Plan()
+        with _on_device(q.device):
+            self._check(self.lib.mvllm_paged_window_attention_plan(
+                *sizes, int(max_query_len), int(max_context_len), window, sinks, *codes, opts_ref,
+                ctypes.byref(plan)))
+            workspace = None
+            if plan.workspace_bytes:
+                workspace = self.workspace(q.device, plan.workspace_bytes)
+            self._check(self.lib.mvllm_paged_window_attention(
+                out.data_ptr(), q.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
+                _ptr(k_scale), _ptr(v_scale), block_tables.data_ptr(), cu_seqlens_q.data_ptr(),
+                context_lens.data_ptr(), seq_lens.data_ptr(), *sizes, num_blocks,
+                block_tables.shape[1], int(max_query_len), int(max_context_len), window, sinks,
+                float(scale), *codes, opts_ref, _ptr(workspace),
+                0 if workspace is None else workspace.numel(), _stream(q.device)))
         return out
 
     @staticmethod

@@ -22,6 +22,13 @@ plus ops that fuse what the reference's caller does in several calls:
     paged_decode_qk_norm_rope(...)             a decode step's qk_norm_rope_kv_write and
                                                paged_attention in one launch (71-95)
 
+and, beside the reference's attention, that of a rolling cache:
+
+    paged_window_attention(q, key_pool, value_pool, block_tables, cu_seqlens_q,
+                    context_lens, seq_lens, max_query_len, max_context_len, window,
+                    sinks=0, scale=None, use_cuda=False)   a sliding window, and the
+                                               sequence's first tokens (sinks)
+
 The callee behind ``use_cuda=True`` is ``libminivllm_hip.so`` (HIP for gfx950).
 
 Routing follows the reference (ops.py:82-89): ``use_cuda=True`` means "use a kernel
@@ -69,6 +76,7 @@ __all__ = [
     "pack_weight",
     "paged_attention",
     "paged_decode_qk_norm_rope",
+    "paged_window_attention",
     "qk_norm_rope",
     "qk_norm_rope_kv_write",
     "rmsnorm",
@@ -647,6 +655,53 @@ def paged_attention(
         q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens, scale,
         k_scale=k_scale, v_scale=v_scale,
     )
+
+
+def paged_window_attention(
+    q: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    context_lens: torch.Tensor,
+    seq_lens: torch.Tensor,
+    max_query_len: int,
+    max_context_len: int,
+    window: int,
+    sinks: int = 0,
+    scale: float | None = None,
+    use_cuda: bool = False,
+    *,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_attention` over a sliding window with sinks (no counterpart in the
+    reference). Kernels: the windowed forms of ``csrc/paged_{decode,prefill}.hip``.
+
+    A query at position p (of a sequence of S keys computing L tokens, query r stands at
+    S - L + r) sees the keys ``j <= p`` with ``j > p - window`` or ``j < sinks``: the ``window``
+    newest ones, itself among them, and the sequence's ``sinks`` first. Both may be larger than
+    any context.
+
+    Pages that no query of the call sees are not read, and their table entries may be -1: a
+    server frees a sequence's page once the window has left it (but for the sinks'). K and V
+    must be finite where some query sees them; elsewhere they may hold anything. A decode row
+    of a sequence without keys is zeros.
+    """
+    if int(window) < 1 or int(sinks) < 0:
+        raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if _use_kernel("paged_attention", use_cuda, q) and _served(
+            "paged_window_attention", _kernel_can_page(q, key_pool, value_pool, block_tables,
+                                                       (cu_seqlens_q, context_lens, seq_lens))):
+        return load_extension().paged_window_attention(
+            q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens, seq_lens,
+            int(max_query_len), int(max_context_len), int(window), int(sinks), scale, k_scale,
+            v_scale)
+    return torch_path.paged_window_attention_gathered(
+        q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens, window, sinks, scale,
+        k_scale=k_scale, v_scale=v_scale)
 
 
 def _kernel_can_page(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,

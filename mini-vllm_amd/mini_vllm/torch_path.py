@@ -23,6 +23,7 @@ __all__ = [
     "dequantize_fp8_pool",
     "kv_write",
     "paged_attention_gathered",
+    "paged_window_attention_gathered",
     "rms_norm",
     "rope_tables",
     "silu",
@@ -189,6 +190,52 @@ def paged_attention_gathered(q: torch.Tensor, key_pool: torch.Tensor, value_pool
         probs = softmax(scores + mask, dim=-1)
         attended = (probs @ v).reshape(num_q_heads, L, head_dim)
         out[start:end] = attended.permute(1, 0, 2)
+    return out
+
+
+def paged_window_attention_gathered(q: torch.Tensor, key_pool: torch.Tensor,
+                                    value_pool: torch.Tensor, block_tables: torch.Tensor,
+                                    cu_seqlens_q: torch.Tensor, context_lens: torch.Tensor,
+                                    window: int, sinks: int = 0, scale: float | None = None,
+                                    k_scale: torch.Tensor | None = None,
+                                    v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Per sequence: gather the keys that its queries see (the sinks and every key from the first
+    query's window on), then dense GQA attention under the window's mask, in fp32 and rounded
+    once. Rows behind the last sequence are zeros here."""
+    if q.dim() != 3:
+        raise ValueError(f"expected q shaped T x H_q x D, got {tuple(q.shape)}")
+    num_seqs = context_lens.shape[0]
+    if block_tables.shape[0] != num_seqs or cu_seqlens_q.shape[0] != num_seqs + 1:
+        raise ValueError("metadata disagrees on the sequence count")
+    block_size, num_kv_heads, head_dim = key_pool.shape[1:]
+    num_q_heads = q.shape[1]
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    out = torch.zeros_like(q)
+    for s in range(num_seqs):
+        start, end = int(cu_seqlens_q[s]), int(cu_seqlens_q[s + 1])
+        L, S = end - start, int(context_lens[s])
+        if L == 0 or S == 0:
+            continue
+        if S < L:
+            raise ValueError(f"sequence {s} attends over {S} tokens but computes {L}")
+        first = max(S - L - window + 1, 0)
+        front = min(sinks, first)
+        keys = torch.cat((torch.arange(front), torch.arange(first, S))).to(q.device)
+        ids = block_tables[s].long().to(q.device)[keys // block_size]
+        if int(ids.min()) < 0:
+            raise ValueError(f"sequence {s} sees a key whose page its table does not hold")
+        k = key_pool[ids, keys % block_size].float()                # V x H_k x D
+        v = value_pool[ids, keys % block_size].float()
+        if key_pool.dtype == torch.float8_e4m3fn:
+            k, v = k * k_scale[ids][..., None], v * v_scale[ids][..., None]
+        qs = q[start:end].float().view(L, num_kv_heads, -1, head_dim)
+        scores = torch.einsum("lhgd,vhd->hglv", qs, k) * scale
+        at = torch.arange(S - L, S, device=q.device).unsqueeze(1)
+        seen = (keys <= at) & ((keys > at - window) | (keys < sinks))
+        probs = softmax(scores.masked_fill(~seen, float("-inf")), dim=-1)
+        attended = torch.einsum("hglv,vhd->lhgd", probs, v)
+        out[start:end] = attended.reshape(L, num_q_heads, head_dim).to(q.dtype)
     return out
 
 

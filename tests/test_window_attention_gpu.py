@@ -1,0 +1,199 @@
+"""Windowed attention with sinks on the GPU against the float64 oracle: every kernel behind it, at
+the lengths, windows, sinks and layouts where their edges meet. Pages that no query sees are
+freed in every batch, and the rows of held pages that no query sees hold NaN."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mini_vllm.kernels import ops
+from window_helpers import assert_close, expected, on, rolling_batch
+
+pytestmark = pytest.mark.gpu
+
+DECODES = [(1, 1), (2, 1), (15, 1), (16, 1), (17, 1), (64, 1), (100, 1), (333, 1), (1000, 1)]
+CHUNKS = [(5, 5), (64, 64), (65, 65), (200, 33), (300, 2), (700, 300), (130, 129)]
+MIXED = [(90, 1), (200, 33), (0, 1), (64, 64), (7, 0), (500, 1), (130, 2), (1, 1)]
+WINDOWS = [(1, 0), (1, 1), (7, 4), (16, 16), (17, 0), (63, 17), (64, 64), (100, 1), (333, 5),
+           (5000, 3), (2, 400), (2**40, 2**40)]
+TYPES = [(torch.float32, None), (torch.float16, None), (torch.bfloat16, None),
+         (torch.float32, torch.float8_e4m3fn), (torch.bfloat16, torch.float8_e4m3fn),
+         (torch.float16, torch.float8_e4m3fn)]
+
+
+def call(batch, device, **more):
+    args = {**on(batch, device), **more}
+    return ops.paged_window_attention(**args, use_cuda=True)
+
+
+@pytest.mark.parametrize("dtype,kv_dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+def test_decode(device, window, sinks, dtype, kv_dtype):
+    b = rolling_batch(DECODES, window, sinks, dtype=dtype, kv_dtype=kv_dtype)
+    assert_close(call(b, device), b, f"{window} {sinks}")
+
+
+@pytest.mark.parametrize("dtype,kv_dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+def test_prefill(device, window, sinks, dtype, kv_dtype):
+    b = rolling_batch(CHUNKS, window, sinks, dtype=dtype, kv_dtype=kv_dtype, hq=4, hk=2)
+    assert_close(call(b, device), b, f"{window} {sinks}")
+
+
+LAYOUTS = [(4, 4, 128, 16), (6, 2, 128, 16), (8, 2, 128, 32), (8, 2, 64, 16), (3, 3, 64, 16),
+           (4, 2, 256, 16), (2, 2, 32, 16), (12, 2, 32, 4), (4, 2, 128, 1), (4, 2, 128, 8),
+           (4, 2, 128, 128), (5, 1, 256, 64)]
+
+
+@pytest.mark.parametrize("dtype,kv_dtype", [TYPES[0], TYPES[2], TYPES[4]])
+@pytest.mark.parametrize("hq,hk,d,page", LAYOUTS)
+@pytest.mark.parametrize("window,sinks", [(40, 5), (130, 20)])
+def test_layouts(device, hq, hk, d, page, window, sinks, dtype, kv_dtype):
+    b = rolling_batch(MIXED, window, sinks, dtype=dtype, kv_dtype=kv_dtype, hq=hq, hk=hk, d=d,
+                      page=page, seed=hq * d)
+    assert_close(call(b, device), b, f"{hq}/{hk} {d} page {page}")
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 0.7])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scales(device, dtype, scale):
+    b = rolling_batch(MIXED, 50, 3, dtype=dtype, hq=4, hk=2, scale=scale)
+    assert_close(call(b, device), b, f"scale {scale}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_fp8_scales_that_are_no_powers_of_two(device, dtype):
+    b = rolling_batch(MIXED + CHUNKS, 90, 9, dtype=dtype, kv_dtype=torch.float8_e4m3fn, hq=4, hk=2,
+                      pow2_scales=False)
+    assert_close(call(b, device), b)
+
+
+@pytest.mark.parametrize("schedule", ["stream", "grid"])
+@pytest.mark.parametrize("n", [65, 300])
+def test_many_sequences(device, extension, n, schedule):
+    """More sequences than a wave has lanes, and rows without keys among them."""
+    pairs = [(37 * i % 301, 1) for i in range(n)]
+    b = rolling_batch(pairs, 100, 4, dtype=torch.bfloat16, hq=4, hk=2)
+    options = {"decode_schedule": 1 if schedule == "stream" else 2, "decode_split_tokens": 64}
+    args = on(b, device)
+    got = extension.paged_window_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], 1, b["max_context_len"], 100, 4, b["scale"],
+        plan_options=options)
+    assert_close(got, b, schedule)
+
+
+def test_many_kv_heads_take_the_grid(device):
+    b = rolling_batch(DECODES + [(3000, 1)], 600, 4, dtype=torch.bfloat16, hq=32, hk=32, d=64)
+    assert_close(call(b, device), b)
+
+
+@pytest.mark.parametrize("chunks", [1, 70])
+@pytest.mark.parametrize("kv_dtype", [None, torch.float8_e4m3fn])
+@pytest.mark.parametrize("pieces", [1, 3, 64])
+@pytest.mark.parametrize("schedule", [0, 1, 2])
+def test_prefill_schedules(device, extension, chunks, kv_dtype, pieces, schedule):
+    """The pair kernel's items whole and cut, on the grid and listed, for more sequences than a
+    wave has lanes too."""
+    pairs = [(900, 150)] + [(20 + 3 * i, 2 + i % 5 if i % 3 else 1) for i in range(chunks - 1)]
+    b = rolling_batch(pairs, 400, 7, dtype=torch.bfloat16, kv_dtype=kv_dtype, hq=4, hk=2)
+    args = on(b, device)
+    got = extension.paged_window_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], b["max_query_len"], b["max_context_len"], 400, 7,
+        b["scale"], args["k_scale"], args["v_scale"],
+        plan_options={"prefill_schedule": schedule, "prefill_pieces": pieces,
+                      "prefill_share_tiles": 1, "prefill_piece_pct": 50})
+    assert_close(got, b)
+
+
+@pytest.mark.parametrize("staging", [0, 1])
+def test_long_window_of_a_long_context(device, extension, staging):
+    b = rolling_batch([(9000, 100), (8200, 1)], 4100, 21, dtype=torch.bfloat16, hq=2, hk=1)
+    args = on(b, device)
+    got = extension.paged_window_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], 100, 9000, 4100, 21, b["scale"],
+        plan_options={"prefill_staging": staging})
+    assert_close(got, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_window_past_every_context_equals_full_attention(device, dtype):
+    b = rolling_batch(MIXED[:2] + MIXED[3:4] + MIXED[5:], 10**6, 0, dtype=dtype)
+    args = on(b, device)
+    full = ops.paged_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], b["max_query_len"], b["max_context_len"], b["scale"],
+        use_cuda=True)
+    out, tolerance = expected(b)
+    assert ((call(b, device) - full).double().cpu().abs() <= 2 * tolerance).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pairs", [DECODES, MIXED])
+def test_rows_behind_the_last_sequence_stay(device, extension, pairs, dtype):
+    b = rolling_batch(pairs, 30, 4, dtype=dtype, hq=4, hk=2, spare_rows=5)
+    args = on(b, device)
+    out = torch.full_like(args["q"], 7.0)
+    got = extension.paged_window_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], b["max_query_len"], b["max_context_len"], 30, 4,
+        b["scale"], out=out)
+    assert got is out
+    assert_close(out, b)
+    assert bool((out[-5:] == 7.0).all())
+
+
+def test_misaligned_queries_and_refusals(device, extension):
+    b = on(rolling_batch(MIXED, 30, 4, dtype=torch.bfloat16, hq=4, hk=2), device)
+    shifted = torch.empty(b["q"].numel() + 1, dtype=torch.bfloat16, device=device)[1:].view(b["q"].shape)
+    shifted.copy_(b["q"])
+    assert torch.equal(call(b, device, q=shifted), call(b, device))
+    pool = torch.empty(b["key_pool"].numel() + 1, dtype=torch.bfloat16, device=device)[1:].view(
+        b["key_pool"].shape)
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        call(b, device, key_pool=pool)
+    with pytest.raises(RuntimeError, match="float64"):
+        call(b, device, q=b["q"].double())
+    with pytest.raises(RuntimeError, match="contiguous"):
+        call(b, device, q=b["q"].transpose(0, 1))
+    with pytest.raises(RuntimeError, match="float8 pool"):
+        call(b, device, k_scale=torch.ones(1, device=device), v_scale=torch.ones(1, device=device))
+    with pytest.raises(ValueError, match="window must be >= 1"):
+        call(b, device, window=0)
+    empty = {**b, "q": b["q"][:0], "block_tables": b["block_tables"][:0],
+             "cu_seqlens_q": b["cu_seqlens_q"][:1], "context_lens": b["context_lens"][:0],
+             "seq_lens": b["seq_lens"][:0]}
+    assert call(empty, device).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("pairs", [DECODES, [(900, 150), (64, 64), (90, 1)]])
+def test_captured_and_replayed_on_another_stream(device, pairs):
+    b = on(rolling_batch(pairs, 100, 4, dtype=torch.bfloat16), device)
+    b2 = on(rolling_batch(pairs, 100, 4, dtype=torch.bfloat16, seed=1), device)
+    want = [call(b, device).clone(), call({**b, "q": b2["q"]}, device).clone()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    q = b["q"].clone()
+    with torch.cuda.stream(side):
+        call(b, device, q=q)        # the stream's workspace exists before the capture
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = call(b, device, q=q)
+    for i in (0, 1, 0, 1):
+        q.copy_(b["q"] if i == 0 else b2["q"])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]), f"replay on inputs {i}"
+        call(b2, device)            # eager work between the replays
+        torch.cuda.synchronize()
+
+
+def test_two_calls_give_the_same_bits(device):
+    b = on(rolling_batch(DECODES + CHUNKS, 200, 4, dtype=torch.bfloat16, kv_dtype=torch.float8_e4m3fn), device)
+    first = call(b, device).clone()
+    for _ in range(5):
+        assert torch.equal(call(b, device), first)
