@@ -305,6 +305,31 @@ int mvllm_qk_norm_rope_kv_write(void* q_out, void* key_pool, void* value_pool, c
  * views of the fused q/k/v projection's output pass its width, so the prefill path
  * needs no copies.) */
 
+/* RoPE of q and k and the write of k and v into the paged cache, in one launch: q_out = rope(q),
+ * key_pool[slot_mapping[t]] = rope(k[t]), value_pool[slot_mapping[t]] = v[t]; the rotation as
+ * mvllm_rope's, the write as mvllm_kv_write's (for models without a QK norm, and for fp8 pools,
+ * which mvllm_qk_norm_rope_kv_write does not take). Replaces, for such a caller, the two ropes and
+ * PagedKvPool.write of model/qwen3_paged.py:76-80 and block/kv_pool.py:116-155; no counterpart in
+ * mini_vllm_C.
+ *   q, q_out [num_tokens, num_q_heads, head_dim]; k, v [num_tokens, num_kv_heads, head_dim], all of
+ *   `dtype` (f32, f16, bf16), q, k and v with heads contiguous within a token and their own token
+ *   strides in elements (0: contiguous); positions [num_tokens] int32 or int64, one outside [0,
+ *   max_positions) gives NaN vectors; cos_table, sin_table [max_positions, head_dim] float32;
+ *   slot_mapping and the pools as mvllm_kv_write (a slot outside the pool writes nothing; its
+ *   token's q is still rotated). Every tensor and token 16-byte aligned.
+ * pool_dtype == dtype: bit for bit mvllm_rope and a copy; head_dim a multiple of 16 up to 1024. An
+ * fp8 pool (head_dim 32, 64, 128 or 256): scales, runs and re-encoding as mvllm_kv_write, at most
+ * one run per block and call; K is quantised from the float32 rotation. An infinity saturates and a
+ * NaN is stored as one, neither counting for its block's scale. */
+int mvllm_rope_kv_write(void* q_out, void* key_pool, void* value_pool, float* k_scales,
+                        float* v_scales, const void* q, const void* k, const void* v,
+                        int64_t q_token_stride, int64_t k_token_stride, int64_t v_token_stride,
+                        const void* positions, int32_t positions_bytes, const float* cos_table,
+                        const float* sin_table, int64_t max_positions,
+                        const int32_t* slot_mapping, int32_t num_tokens, int32_t num_q_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                        int64_t num_blocks, int32_t dtype, int32_t pool_dtype, void* stream);
+
 /* A decode step's attention with its new token's QK-norm, RoPE and KV write in the same
  * launch, for a decode-only batch (every sequence computes one token: seq_lens all 1,
  * cu_seqlens_q = 0, 1, ..., num_seqs, so row s is sequence s's) over a float16 or

@@ -24,6 +24,7 @@
 #include "sampling.hpp"
 #include "paged_attention.hpp"
 #include "probe.hpp"
+#include "rope_write.hpp"
 
 namespace {
 
@@ -1419,6 +1420,86 @@ int mvllm_add_rmsnorm(void* h_out, void* out, const void* x, const void* residua
   return hip_status(mvllm::launch_add_rmsnorm(x, residual, weight, h_out, out, rows, dim, eps,
                                               dtype, static_cast<hipStream_t>(stream)),
                     "add_rmsnorm: launch");
+}
+
+int mvllm_rope_kv_write(void* q_out, void* key_pool, void* value_pool, float* k_scales,
+                        float* v_scales, const void* q, const void* k, const void* v,
+                        int64_t q_token_stride, int64_t k_token_stride, int64_t v_token_stride,
+                        const void* positions, int32_t positions_bytes, const float* cos_table,
+                        const float* sin_table, int64_t max_positions,
+                        const int32_t* slot_mapping, int32_t num_tokens, int32_t num_q_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                        int64_t num_blocks, int32_t dtype, int32_t pool_dtype, void* stream) {
+  g_error[0] = '\0';
+  const char* name = "rope_kv_write";
+  if (num_tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_blocks <= 0 ||
+      max_positions <= 0 || !is_pow2(block_size)) {
+    return fail(MVLLM_ERR_INVALID,
+                "%s: bad shape (block size %d must be a power of two, the pool and the cos/sin tables "
+                "not empty)",
+                name, block_size);
+  }
+  if (positions_bytes != 4 && positions_bytes != 8) {
+    return fail(MVLLM_ERR_INVALID, "%s: positions must be int32 or int64", name);
+  }
+  if (!mvllm::rope_write_supported(dtype, pool_dtype, head_dim)) {
+    return fail(MVLLM_ERR_UNSUPPORTED,
+                "%s: dtype code %d into a pool of code %d at head dim %d is not served (float32, "
+                "float16 and bfloat16 into a pool of their own type with a head dim that is a multiple "
+                "of 16 up to 1024, or into float8_e4m3fn with 32, 64, 128 or 256)",
+                name, dtype, pool_dtype, head_dim);
+  }
+  const bool fp8 = pool_dtype == mvllm::kFP8E4M3;
+  if (fp8 != (k_scales != nullptr && v_scales != nullptr) || (!fp8 && (k_scales || v_scales))) {
+    return fail(MVLLM_ERR_INVALID,
+                "%s: k_scales and v_scales are required for a float8 pool and only for one", name);
+  }
+  if (num_tokens == 0) return MVLLM_OK;
+  if (q_out == nullptr || key_pool == nullptr || value_pool == nullptr || q == nullptr || k == nullptr ||
+      v == nullptr || positions == nullptr || cos_table == nullptr || sin_table == nullptr ||
+      slot_mapping == nullptr) {
+    return fail(MVLLM_ERR_INVALID, "%s: a required pointer is NULL", name);
+  }
+  uintptr_t bits = 0;
+  for (const void* ptr : {static_cast<const void*>(q_out), static_cast<const void*>(key_pool),
+                          static_cast<const void*>(value_pool), q, k, v,
+                          static_cast<const void*>(cos_table), static_cast<const void*>(sin_table)}) {
+    bits |= reinterpret_cast<uintptr_t>(ptr);
+  }
+  mvllm::RopeWriteParams p{};
+  const int64_t elem = element_bytes(dtype);
+  const int64_t q_row = static_cast<int64_t>(num_q_heads) * head_dim;
+  const int64_t kv_row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  p.q_stride = q_token_stride > 0 ? q_token_stride : q_row;
+  p.k_stride = k_token_stride > 0 ? k_token_stride : kv_row;
+  p.v_stride = v_token_stride > 0 ? v_token_stride : kv_row;
+  if (p.q_stride < q_row || p.k_stride < kv_row || p.v_stride < kv_row) {
+    return fail(MVLLM_ERR_INVALID, "%s: a token stride must cover the token's heads", name);
+  }
+  if (bits % 16 != 0 || ((p.q_stride | p.k_stride | p.v_stride) * elem) % 16 != 0) {
+    return fail(MVLLM_ERR_INVALID, "%s: every tensor and token must be 16-byte aligned", name);
+  }
+  p.q_out = q_out;
+  p.k_pool = key_pool;
+  p.v_pool = value_pool;
+  p.k_scales = k_scales;
+  p.v_scales = v_scales;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.positions = positions;
+  p.cos_t = cos_table;
+  p.sin_t = sin_table;
+  p.slots = slot_mapping;
+  p.num_blocks = num_blocks;
+  p.max_positions = max_positions;
+  p.tokens = num_tokens;
+  p.hq = num_q_heads;
+  p.hk = num_kv_heads;
+  while ((1 << p.block_shift) < block_size) ++p.block_shift;
+  return hip_status(mvllm::launch_rope_write(p, dtype, pool_dtype, head_dim, positions_bytes,
+                                             static_cast<hipStream_t>(stream)),
+                    "rope_kv_write: launch");
 }
 
 int mvllm_embed_rmsnorm(void* h_out, void* out, const void* table, int64_t vocab,

@@ -71,7 +71,7 @@ HIP_FLAGS = [
 # to compile to the same bits (measured: contraction left on there moved one in ten
 # float16 rows by an ulp, and the decode ran no faster).
 EXTRA_FLAGS = {"elementwise.hip": ["-ffp-contract=off"], "linear.hip": ["-ffp-contract=off"],
-               "paged_decode.hip": ["-ffp-contract=off"]}
+               "paged_decode.hip": ["-ffp-contract=off"], "rope_write.hip": ["-ffp-contract=off"]}
 
 # hipBLASLt (csrc/blas.hip). Its soname is the one torch's bundled copy carries, so in a
 # process that has imported torch the library binds to that copy.
@@ -394,6 +394,9 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.mvllm_paged_decode_qk_norm_rope.argtypes = (
         [p] * 4 + [i64, i64] + [p] * 4 + [i64, f32] + [p] * 6 + [i32] * 5
         + [i64, i32, i32, f32, i32, opts, p, u64, p])
+    lib.mvllm_rope_kv_write.restype = ctypes.c_int
+    lib.mvllm_rope_kv_write.argtypes = (
+        [p] * 8 + [i64] * 3 + [p, i32, p, p, i64, p] + [i32] * 5 + [i64, i32, i32, p])
     lib.mvllm_kv_write.restype = ctypes.c_int
     lib.mvllm_kv_write.argtypes = [p] * 7 + [i32] * 4 + [i64, i32, i32, p]
     lib.mvllm_argmax.restype = ctypes.c_int
@@ -452,6 +455,7 @@ EXPORTED_SYMBOLS = (
     "mvllm_embed_rmsnorm",
     "mvllm_axpby",
     "mvllm_kv_write",
+    "mvllm_rope_kv_write",
     "mvllm_qk_norm_rope",
     "mvllm_argmax",
     "mvllm_qk_norm_rope_kv_write",
@@ -1172,6 +1176,78 @@ class HipExtension:
             key_pool.shape[0] * key_pool.shape[1],
             q.shape[0], q.shape[1], k.shape[1], d, positions.numel(), cos.shape[0], float(eps),
             q.stride(0), k.stride(0), code, _stream(q.device)))
+        return q_out
+
+    def rope_kv_write(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                      key_pool: torch.Tensor, value_pool: torch.Tensor,
+                      slot_mapping: torch.Tensor, k_scale: torch.Tensor | None = None,
+                      v_scale: torch.Tensor | None = None) -> torch.Tensor:
+        """RoPE of q and k at each token's position, k and v written to their slots of the
+        layer's pools, in one launch; returns the rotated q. q, k and v may be column views of
+        one projection's output."""
+        name = "rope_kv_write"
+        tensors = [q, k, v, positions, cos, sin, key_pool, value_pool, slot_mapping]
+        tensors += [s for s in (k_scale, v_scale) if s is not None]
+        if not all(t.is_cuda and t.device == q.device for t in tensors):
+            raise RuntimeError(f"{name}: every tensor must be on q's CUDA device")
+        if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] \
+                or q.shape[2] != k.shape[2]:
+            raise RuntimeError(
+                f"{name}: q must be T x H_q x D and k, v T x H_k x D, got {tuple(q.shape)}, "
+                f"{tuple(k.shape)} and {tuple(v.shape)}")
+        tokens, hq, d = q.shape
+        hk = k.shape[1]
+        if k.dtype != q.dtype or v.dtype != q.dtype or q.dtype not in (
+                torch.float32, torch.float16, torch.bfloat16):
+            raise RuntimeError(f"{name}: q, k and v must share float32, float16 or bfloat16, got "
+                               f"{q.dtype}, {k.dtype} and {v.dtype}")
+        fp8 = key_pool.dtype == torch.float8_e4m3fn
+        if key_pool.dtype != value_pool.dtype or (key_pool.dtype != q.dtype and not fp8):
+            raise RuntimeError(f"{name}: the pools must be of q's dtype or float8_e4m3fn, got "
+                               f"{key_pool.dtype} and {value_pool.dtype}")
+        if key_pool.dim() != 4 or key_pool.shape != value_pool.shape \
+                or tuple(key_pool.shape[2:]) != (hk, d) \
+                or not (key_pool.is_contiguous() and value_pool.is_contiguous()):
+            raise RuntimeError(f"{name}: the pools must be contiguous num_blocks x P x {hk} x {d}, "
+                               f"got {tuple(key_pool.shape)} and {tuple(value_pool.shape)}")
+        num_blocks, block_size = key_pool.shape[:2]
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape \
+                or cos.dim() != 2 or cos.shape[1] != d:
+            raise RuntimeError(f"{name}: the cos/sin tables must be float32 max_pos x {d}")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,):
+            raise RuntimeError(f"{name}: positions must be an int32 or int64 [{tokens}]")
+        if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (tokens,):
+            raise RuntimeError(f"{name}: slot_mapping must be an int32 [{tokens}]")
+        if fp8:
+            for what, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+                if s is None or s.dtype != torch.float32 or tuple(s.shape) != (num_blocks, hk) \
+                        or not s.is_contiguous():
+                    raise RuntimeError(f"{name}: a float8_e4m3fn pool needs a contiguous float32 "
+                                       f"{num_blocks} x {hk} {what}")
+        elif k_scale is not None or v_scale is not None:
+            raise RuntimeError(f"{name}: k_scale/v_scale apply only to a float8 pool")
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if tokens == 0:
+            return q_out
+
+        def rows(t):  # heads contiguous within each token, every token 16-byte aligned
+            size = t.element_size()
+            if t.stride(2) == 1 and (t.stride(1) == d or t.shape[1] == 1) \
+                    and (t.stride(0) >= t.shape[1] * d or tokens == 1) \
+                    and t.stride(0) * size % 16 == 0 and t.data_ptr() % 16 == 0:
+                return t
+            return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+        q, k, v, cos, sin = rows(q), rows(k), rows(v), cos.contiguous(), sin.contiguous()
+        positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
+        stride = [t.stride(0) if tokens > 1 else 0 for t in (q, k, v)]
+        with _on_device(q.device):
+            self._check(self.lib.mvllm_rope_kv_write(
+                q_out.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(), _ptr(k_scale),
+                _ptr(v_scale), q.data_ptr(), k.data_ptr(), v.data_ptr(), *stride,
+                positions.data_ptr(), positions.element_size(), cos.data_ptr(), sin.data_ptr(),
+                cos.shape[0], slot_mapping.data_ptr(), tokens, hq, hk, d, block_size, num_blocks,
+                DTYPE_CODES[q.dtype], DTYPE_CODES[key_pool.dtype], _stream(q.device)))
         return q_out
 
     def swiglu_interleaved(self, gate_up: torch.Tensor) -> torch.Tensor:

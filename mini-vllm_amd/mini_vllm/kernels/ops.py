@@ -22,8 +22,11 @@ plus ops that fuse what the reference's caller does in several calls:
     paged_decode_qk_norm_rope(...)             a decode step's qk_norm_rope_kv_write and
                                                paged_attention in one launch (71-95)
 
-and, beside the reference's attention, that of a rolling cache:
+and, beside the reference's, a rolling cache's append and attention:
 
+    rope_kv_write(q, k, v, positions, cos, sin, key_pool, value_pool, slot_mapping,
+                  use_cuda=False)              the rotation and the KV write in one launch,
+                                               without a QK norm or into an fp8 pool
     paged_window_attention(q, key_pool, value_pool, block_tables, cu_seqlens_q,
                     context_lens, seq_lens, max_query_len, max_context_len, window,
                     sinks=0, scale=None, use_cuda=False)   a sliding window, and the
@@ -81,6 +84,7 @@ __all__ = [
     "qk_norm_rope_kv_write",
     "rmsnorm",
     "rope",
+    "rope_kv_write",
     "sampling_probabilities",
     "set_strict",
     "strict_kernels",
@@ -745,6 +749,43 @@ def kv_write(key_pool: torch.Tensor, value_pool: torch.Tensor, key: torch.Tensor
         return
     torch_path.kv_write(key_pool, value_pool, key, value, slot_mapping,
                         k_scale=k_scale, v_scale=v_scale)
+
+
+def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                  cos: torch.Tensor, sin: torch.Tensor, key_pool: torch.Tensor,
+                  value_pool: torch.Tensor, slot_mapping: torch.Tensor, use_cuda: bool = False, *,
+                  k_scale: torch.Tensor | None = None,
+                  v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """The append of a step's tokens: RoPE of ``q`` (T x H_q x D) and ``k`` (T x H_k x D) at
+    ``positions`` (T), the rotated k and ``v`` written to ``slot_mapping`` of one layer's pools
+    (as :func:`kv_write`; a negative slot writes nothing), the rotated q returned. Kernel:
+    ``csrc/rope_write.hip``, one launch.
+
+    For models without a QK norm, and for fp8 pools (:func:`qk_norm_rope_kv_write` serves
+    neither). A pool of q's dtype gets the bits of :func:`rope` then :func:`kv_write`; a
+    ``float8_e4m3fn`` one is quantised by the same policy from the float32 rotation, not rounded
+    to k's dtype between. q, k and v may be column views of one projection's output."""
+    if _use_kernel("kv_write", use_cuda, q) and _served("rope_kv_write", _rope_kv_write_reason(
+            q, k, v, positions, cos, sin, key_pool, value_pool, slot_mapping)):
+        return load_extension().rope_kv_write(q, k, v, positions, cos, sin, key_pool, value_pool,
+                                              slot_mapping, k_scale, v_scale)
+    return torch_path.rope_kv_write(q, k, v, positions, cos, sin, key_pool, value_pool,
+                                    slot_mapping, k_scale=k_scale, v_scale=v_scale)
+
+
+def _rope_kv_write_reason(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                          positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                          key_pool: torch.Tensor, value_pool: torch.Tensor,
+                          slot_mapping: torch.Tensor) -> str | None:
+    reason = _kv_write_reason(key_pool, value_pool, k, v, slot_mapping) or _rope_reason(q, cos, sin)
+    if reason is not None:
+        return reason
+    if not all(t.is_cuda for t in (k, positions, cos, sin)):
+        return "k, the positions and the cos/sin tables must be device tensors"
+    d = q.shape[-1]
+    if key_pool.dtype == torch.float8_e4m3fn:
+        return None if d in PAGED_HEAD_DIMS else f"head dim {d} is not served for an fp8 pool"
+    return None if d % 16 == 0 and d <= 1024 else f"head dim {d} is not a multiple of 16 up to 1024"
 
 
 def _kv_write_reason(key_pool: torch.Tensor, value_pool: torch.Tensor, key: torch.Tensor,

@@ -25,6 +25,7 @@ __all__ = [
     "paged_attention_gathered",
     "paged_window_attention_gathered",
     "rms_norm",
+    "rope_kv_write",
     "rope_tables",
     "silu",
     "softmax",
@@ -125,6 +126,30 @@ def kv_write(key_pool: torch.Tensor, value_pool: torch.Tensor, key: torch.Tensor
             pool[block, row0:row0 + n] = enc.to(torch.float8_e4m3fn)
             scales[block] = s
         t += n
+
+
+def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                  cos: torch.Tensor, sin: torch.Tensor, key_pool: torch.Tensor,
+                  value_pool: torch.Tensor, slot_mapping: torch.Tensor, *,
+                  k_scale: torch.Tensor | None = None,
+                  v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate q and k, write k and v (:func:`kv_write`); the rotated q. An fp8 pool is
+    quantised from k's float32 rotation; a value that is not finite is stored for itself (an
+    infinity saturated), with no part in its page's scale."""
+    turned = apply_rope(k.float(), positions, cos, sin)
+    if key_pool.dtype != torch.float8_e4m3fn:
+        kv_write(key_pool, value_pool, turned.to(k.dtype), v, slot_mapping)
+    else:
+        v = v.float()
+        kv_write(key_pool, value_pool, torch.where(turned.isfinite(), turned, 0.0),
+                 torch.where(v.isfinite(), v, 0.0), slot_mapping, k_scale=k_scale, v_scale=v_scale)
+        keep = slot_mapping >= 0
+        slots = slot_mapping[keep].to(torch.int64)
+        for pool, x in ((key_pool, turned[keep]), (value_pool, v[keep])):
+            at, head, e = (~x.isfinite()).nonzero(as_tuple=True)
+            flat = pool.view(-1, *pool.shape[2:])
+            flat[slots[at], head, e] = x[at, head, e].clamp(-448.0, 448.0).to(pool.dtype)
+    return apply_rope(q, positions, cos, sin)
 
 
 def dequantize_fp8_pool(pool: torch.Tensor, scales: torch.Tensor,
