@@ -247,10 +247,12 @@ def held_values(pool, scale):
     return pool.to(torch.bfloat16) * scale.to(torch.bfloat16)[:, None, :, None]
 
 
+PACKAGE = str(Path(__file__).resolve().parent.parent / "mini-vllm_amd")
+
+
 def the_ops():
-    package = str(Path(__file__).resolve().parent.parent / "mini-vllm_amd")
-    if package not in sys.path:
-        sys.path.insert(0, package)
+    if "mini_vllm" not in sys.modules:
+        sys.path.insert(0, PACKAGE)
     from mini_vllm.kernels import ops
 
     return ops
