@@ -833,6 +833,7 @@ int paged_attention_entry(const char* name, void* out, const void* q, const void
   p.scale = scale;
   p.window = win.window;
   p.sinks = win.sinks;
+  p.last_block = static_cast<uint32_t>(num_blocks < INT32_MAX ? num_blocks - 1 : INT32_MAX - 1);
   return launch_planned(plan, p, workspace, q_dtype, kv_dtype, head_dim, max_query_len,
                         static_cast<hipStream_t>(stream), name);
 }

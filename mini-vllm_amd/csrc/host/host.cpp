@@ -34,6 +34,9 @@ using BytesFn = decltype(&mvllm_linear_workspace_bytes);
 using SwigluFn = decltype(&mvllm_linear_swiglu);
 using NormFn = decltype(&mvllm_linear_residual_rmsnorm);
 using ErrorFn = decltype(&mvllm_last_error);
+using WindowPlanFn = decltype(&mvllm_paged_window_attention_plan);
+using WindowFn = decltype(&mvllm_paged_window_attention);
+using RopeWriteFn = decltype(&mvllm_rope_kv_write);
 
 // One library's entries; the extension object that loaded the library holds them as a capsule.
 struct Entries {
@@ -50,6 +53,20 @@ constexpr const char* kCapsule = "mvllm_host.entries";
 
 const Entries* entries_of(PyObject* o) {
   return static_cast<const Entries*>(PyCapsule_GetPointer(o, kCapsule));
+}
+
+// The rolling cache's: windowed attention and the rotating append, a capsule of their own.
+struct RollingEntries {
+  WindowPlanFn plan;
+  WindowFn window;
+  RopeWriteFn rope_write;
+  ErrorFn error;
+};
+
+constexpr const char* kRollingCapsule = "mvllm_host.rolling_entries";
+
+const RollingEntries* rolling_entries_of(PyObject* o) {
+  return static_cast<const RollingEntries*>(PyCapsule_GetPointer(o, kRollingCapsule));
 }
 
 // An active dispatch or function mode sees the Python path's calls; it has none to see here.
@@ -127,7 +144,8 @@ uint64_t bytes(const at::Tensor& t) { return t.defined() ? static_cast<uint64_t>
 
 PyObject* none() { Py_RETURN_NONE; }
 
-PyObject* finish(const Entries* e, int rc, PyObject* result) {
+template <typename E>
+PyObject* finish(const E* e, int rc, PyObject* result) {
   if (rc == 0) return result;
   Py_XDECREF(result);
   const char* message = e->error();
@@ -333,6 +351,147 @@ PyObject* paged_decode_qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t
   END_HANDLE_TH_ERRORS
 }
 
+bool current(int device) { return device == static_cast<int>(c10::hip::current_device()); }
+
+// (entries, workspaces, q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens,
+//  seq_lens, max_query_len, max_context_len, window, sinks, scale, k_scale, v_scale)
+PyObject* paged_window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 16 || !PyDict_CheckExact(args[1]) || modes()) return none();
+  const RollingEntries* e = rolling_entries_of(args[0]);
+  if (e == nullptr) return nullptr;
+  PyObject* const* a = args + 2;
+  Paged p;
+  int64_t window, sinks;
+  p.q = tensor(a[0]);
+  p.kp = tensor(a[1]);
+  p.vp = tensor(a[2]);
+  p.tables = tensor(a[3]);
+  p.cu = tensor(a[4]);
+  p.ctx = tensor(a[5]);
+  p.lens = tensor(a[6]);
+  if (!integer(a[7], p.max_q) || !integer(a[8], p.max_ctx) || !integer(a[9], window) ||
+      !integer(a[10], sinks) || !number(a[11], p.scale) || !optional(a[12], p.ks) ||
+      !optional(a[13], p.vs) || !p.check(true) || !aligned(*p.q) || !aligned(*p.kp) ||
+      !aligned(*p.vp) || !current(p.device)) {
+    return none();
+  }
+  const auto tokens = static_cast<int32_t>(p.q->size(0)), seqs = static_cast<int32_t>(p.lens->size(0)),
+             hq = static_cast<int32_t>(p.q->size(1)), hk = static_cast<int32_t>(p.kp->size(2)),
+             d = static_cast<int32_t>(p.q->size(2)), page = static_cast<int32_t>(p.kp->size(1)),
+             max_q = static_cast<int32_t>(p.max_q), max_ctx = static_cast<int32_t>(p.max_ctx),
+             win = static_cast<int32_t>(window), front = static_cast<int32_t>(sinks);
+  mvllm_paged_plan plan;
+  if (e->plan(tokens, seqs, hq, hk, d, page, max_q, max_ctx, win, front, p.q_code, p.kv_code, nullptr,
+              &plan) != 0) {
+    return none();
+  }
+  void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(p.device)).stream();
+  at::Tensor ws;
+  if (plan.workspace_bytes > 0 && !workspace(args[1], p.device, stream, plan.workspace_bytes, ws)) {
+    return none();
+  }
+  at::Tensor out = at::empty(p.q->sizes(), p.q->options());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = e->window(out.data_ptr(), p.q->data_ptr(), p.kp->data_ptr(), p.vp->data_ptr(),
+                 p.ks ? static_cast<const float*>(p.ks->data_ptr()) : nullptr,
+                 p.vs ? static_cast<const float*>(p.vs->data_ptr()) : nullptr,
+                 static_cast<const int32_t*>(p.tables->data_ptr()),
+                 static_cast<const int32_t*>(p.cu->data_ptr()),
+                 static_cast<const int32_t*>(p.ctx->data_ptr()),
+                 static_cast<const int32_t*>(p.lens->data_ptr()), tokens, seqs, hq, hk, d, page,
+                 p.kp->size(0), static_cast<int32_t>(p.tables->size(1)), max_q, max_ctx, win, front,
+                 static_cast<float>(p.scale), p.q_code, p.kv_code, nullptr, pointer(ws), bytes(ws),
+                 stream);
+  Py_END_ALLOW_THREADS
+  return finish(e, rc, rc == 0 ? THPVariable_Wrap(std::move(out)) : nullptr);
+  END_HANDLE_TH_ERRORS
+}
+
+// (entries, q, k, v, positions, cos, sin, key_pool, value_pool, slot_mapping, k_scale, v_scale)
+PyObject* rope_kv_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12 || modes()) return none();
+  const RollingEntries* e = rolling_entries_of(args[0]);
+  if (e == nullptr) return nullptr;
+  PyObject* const* a = args + 1;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *pos = tensor(a[3]),
+                   *cos = tensor(a[4]), *sin = tensor(a[5]), *kp = tensor(a[6]), *vp = tensor(a[7]),
+                   *slots = tensor(a[8]), *ks = nullptr, *vs = nullptr;
+  if (!q || !k || !v || !pos || !cos || !sin || !kp || !vp || !slots || !optional(a[9], ks) ||
+      !optional(a[10], vs)) {
+    return none();
+  }
+  if (q->dim() != 3 || k->dim() != 3 || kp->dim() != 4 || v->sizes() != k->sizes() ||
+      vp->sizes() != kp->sizes() || k->size(0) != q->size(0) || k->size(2) != q->size(2) ||
+      kp->size(2) != k->size(1) || kp->size(3) != k->size(2) || !kp->is_contiguous() ||
+      !vp->is_contiguous()) {
+    return none();
+  }
+  const int64_t tokens = q->size(0), hq = q->size(1), hk = k->size(1), d = q->size(2), page = kp->size(1);
+  const int code = code_of(q->scalar_type()), pool_code = code_of(kp->scalar_type());
+  const bool fp8 = pool_code == MVLLM_DTYPE_FP8_E4M3;
+  if (code < 0 || code == MVLLM_DTYPE_FP8_E4M3 || k->scalar_type() != q->scalar_type() ||
+      v->scalar_type() != q->scalar_type() || vp->scalar_type() != kp->scalar_type() ||
+      (!fp8 && pool_code != code) || fp8 != (ks != nullptr) || fp8 != (vs != nullptr)) {
+    return none();
+  }
+  if (tokens < 1 || tokens >= INT32_MAX || hq < 1 || hk < 1 || d < 1 || page < 1 || page >= INT32_MAX ||
+      (fp8 ? d != 32 && d != 64 && d != 128 && d != 256 : d % 16 != 0 || d > 1024)) {
+    return none();
+  }
+  const int64_t elem = q->element_size();
+  for (const at::Tensor* t : {q, k, v}) {  // heads contiguous within each token, tokens aligned
+    if (t->stride(2) != 1 || t->stride(1) != d || t->stride(0) < t->size(1) * d ||
+        t->stride(0) * elem % 16 != 0 || !aligned(*t)) {
+      return none();
+    }
+  }
+  for (const at::Tensor* t : {cos, sin}) {
+    if (t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(1) != d || t->size(0) < 1 ||
+        t->size(0) != cos->size(0) || !t->is_contiguous() || !aligned(*t)) {
+      return none();
+    }
+  }
+  const int64_t pos_bytes = pos->element_size();
+  if ((pos->scalar_type() != at::kLong && pos->scalar_type() != at::kInt) || pos->dim() != 1 ||
+      pos->size(0) != tokens || !pos->is_contiguous() || slots->scalar_type() != at::kInt ||
+      slots->dim() != 1 || slots->size(0) != tokens || !slots->is_contiguous() || !aligned(*kp) ||
+      !aligned(*vp)) {
+    return none();
+  }
+  const int device = q->get_device();
+  for (const at::Tensor* t : {k, v, pos, cos, sin, kp, vp, slots}) {
+    if (t->get_device() != device) return none();
+  }
+  if (!current(device)) return none();
+  if (fp8) {
+    for (const at::Tensor* t : {ks, vs}) {
+      if (t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(0) != kp->size(0) ||
+          t->size(1) != hk || !t->is_contiguous() || t->get_device() != device) {
+        return none();
+      }
+    }
+  }
+  void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+  at::Tensor out = at::empty(q->sizes(), q->options());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = e->rope_write(out.data_ptr(), kp->data_ptr(), vp->data_ptr(),
+                     fp8 ? static_cast<float*>(ks->data_ptr()) : nullptr,
+                     fp8 ? static_cast<float*>(vs->data_ptr()) : nullptr, q->data_ptr(), k->data_ptr(),
+                     v->data_ptr(), q->stride(0), k->stride(0), v->stride(0), pos->data_ptr(),
+                     static_cast<int32_t>(pos_bytes), static_cast<const float*>(cos->data_ptr()),
+                     static_cast<const float*>(sin->data_ptr()), cos->size(0),
+                     static_cast<const int32_t*>(slots->data_ptr()), static_cast<int32_t>(tokens),
+                     static_cast<int32_t>(hq), static_cast<int32_t>(hk), static_cast<int32_t>(d),
+                     static_cast<int32_t>(page), kp->size(0), code, pool_code, stream);
+  Py_END_ALLOW_THREADS
+  return finish(e, rc, rc == 0 ? THPVariable_Wrap(std::move(out)) : nullptr);
+  END_HANDLE_TH_ERRORS
+}
+
 // x [m, k] against a packed weight of n rows: the skinny kernels take it as it is.
 bool skinny(const at::Tensor* x, const at::Tensor* w, int64_t n) {
   if (!x || !w || x->dim() != 2 || !sixteen_bit(*x) || w->scalar_type() != x->scalar_type() ||
@@ -429,10 +588,25 @@ PyObject* entries(PyObject*, PyObject* args) {
   return capsule;
 }
 
+// A capsule of the rolling cache's entries: plan, windowed attention, append, the error text.
+PyObject* rolling_entries(PyObject*, PyObject* args) {
+  unsigned long long f[4];
+  if (!PyArg_ParseTuple(args, "KKKK", &f[0], &f[1], &f[2], &f[3])) return nullptr;
+  auto* e = new RollingEntries{reinterpret_cast<WindowPlanFn>(f[0]), reinterpret_cast<WindowFn>(f[1]),
+                               reinterpret_cast<RopeWriteFn>(f[2]), reinterpret_cast<ErrorFn>(f[3])};
+  PyObject* capsule = PyCapsule_New(e, kRollingCapsule, [](PyObject* c) {
+    delete static_cast<RollingEntries*>(PyCapsule_GetPointer(c, kRollingCapsule));
+  });
+  if (capsule == nullptr) delete e;
+  return capsule;
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(name), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     {"entries", entries, METH_VARARGS, nullptr}, FAST(paged_served),   FAST(paged_attention),
     FAST(paged_decode_qk_norm_rope),       FAST(linear_swiglu),  FAST(linear_residual_rmsnorm),
+    {"rolling_entries", rolling_entries, METH_VARARGS, nullptr}, FAST(paged_window_attention),
+    FAST(rope_kv_write),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "mvllm_host", nullptr, -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

@@ -221,7 +221,16 @@ struct PagedParams {
   int window;         // > 0: windowed attention (the kernels' kWindow forms): a query at
   int sinks;          // position p sees the keys j <= p with j > p - window or j < sinks
                       // (sinks + window < 2^31)
+  uint32_t last_block;  // windowed: the pool's last page, which an id outside the pool is read as
 };
+
+// A block table's entry as a page of the pool. A rolling cache's tables hold -1 where pages were
+// freed; should a call see such a key all the same (a larger window than the caller freed for), what
+// it gets is meaningless, but nothing outside the pool is read.
+__device__ __forceinline__ int held_page(const PagedParams& p, int id) {
+  const uint32_t u = static_cast<uint32_t>(id);
+  return static_cast<int>(u < p.last_block ? u : p.last_block);
+}
 
 // Windowed attention. The keys that the queries of a work item see are the sinks and one range
 // that ends at the last query's position, so an item walks them as a list without the keys

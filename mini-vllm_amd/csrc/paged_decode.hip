@@ -191,9 +191,11 @@ template <> struct Query<f16_t, fp8_t> : PackedQuery<f16_t, fp8_t> {};
 // Where the entries of a sequence's key list lie: all positions in order, or for windowed
 // attention the sinks and then, `gap` positions on, the window's keys.
 struct EveryKey {
+  static constexpr bool kListed = false;
   __device__ int operator()(int v) const { return v; }
 };
 struct WindowKeys {
+  static constexpr bool kListed = true;
   int sinks, gap;
   __device__ int operator()(int v) const { return v < sinks ? v : v + gap; }
 };
@@ -301,6 +303,8 @@ struct Decode {
         int tok = t0 + u * RG + g;
         valid[u] = tok < se;
         tok = valid[u] ? tok : se - 1;
+        // (here and not where the ids are requested, which would wait for them there)
+        if constexpr (Keys::kListed) pg[u] = held_page(p, pg[u]);
         const int64_t slot = (static_cast<int64_t>(pg[u]) << p.table_shift) + (at(tok) & p.block_mask);
         const int64_t off = slot * p.kv_row_bytes + kvh * p.kv_head_bytes + r * E * kElemBytes;
         kw[u] = load16_stream(kbase + off);

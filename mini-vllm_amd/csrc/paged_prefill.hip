@@ -609,6 +609,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     if (u1 <= 0) return;
   }
   auto position = [&](int v) __attribute__((always_inline)) { return kWindow ? list_position(list, v) : v; };
+  auto held = [&](int id) __attribute__((always_inline)) { return kWindow ? held_page(p, id) : id; };
   auto advance = [&](Cursor& k) __attribute__((always_inline)) {
     ++k.u;
     if (++k.t < k.nt) return;
@@ -660,11 +661,11 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     }
     if constexpr (kFp8) {
 #pragma unroll
-      for (int u = 0; u < kKUnits; ++u) ksc[S][u] = p.k_scales[static_cast<int64_t>(kpg[S][u]) * p.hk + kvh];
+      for (int u = 0; u < kKUnits; ++u) ksc[S][u] = p.k_scales[static_cast<int64_t>(held(kpg[S][u])) * p.hk + kvh];
 #pragma unroll
       for (int u = 0; u < kVUnits; ++u) {
 #pragma unroll
-        for (int j = 0; j < kVKeys; ++j) vsc[S][u][j] = p.v_scales[static_cast<int64_t>(vpg[S][u][j]) * p.hk + kvh];
+        for (int j = 0; j < kVKeys; ++j) vsc[S][u][j] = p.v_scales[static_cast<int64_t>(held(vpg[S][u][j])) * p.hk + kvh];
       }
     }
   };
@@ -686,7 +687,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
 #pragma unroll
     for (int u = 0; u < kKUnits; ++u) {
       const int key = position(min(key0 + k_key(u), last));
-      const uint64_t off = pool_offset(kpg[S][u], key, head_off + k_dim(u) * kElemBytes);
+      const uint64_t off = pool_offset(held(kpg[S][u]), key, head_off + k_dim(u) * kElemBytes);
       kreg[S][u] = Stage<TQ, TKV>::load(kpool + off, kFp8 ? ksc[S][u] : 1.0f);
     }
 #pragma unroll
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
 #pragma unroll
       for (int j = 0; j < kVKeys; ++j) {
         const int key = position(min(key0 + kVKeys * v_grp(u) + j, last));
-        const uint64_t off = pool_offset(vpg[S][u][j], key, head_off + v_dim(u) * kElemBytes);
+        const uint64_t off = pool_offset(held(vpg[S][u][j]), key, head_off + v_dim(u) * kElemBytes);
         vreg[S][u][j] = Stage<TQ, TKV>::load(vpool + off, kFp8 ? vsc[S][u][j] : 1.0f);
       }
     }
@@ -1576,6 +1577,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
     int at = min(tile * kTileKeys + KW * wave, context - 1);
     if constexpr (kWindow) at = list_position(list, at);
     pages = load_dword_now(table + (at >> p.block_shift));
+    if constexpr (kWindow) pages = held_page(p, pages);
     if constexpr (kFp8) {
       const int64_t si = static_cast<int64_t>(pages) * p.hk + kvh;
       ks_lane = __int_as_float(load_dword_now(p.k_scales + si));

@@ -544,6 +544,10 @@ class HipExtension:
                 lib.mvllm_paged_decode_qk_norm_rope, lib.mvllm_linear_workspace_bytes,
                 lib.mvllm_linear_swiglu, lib.mvllm_linear_residual_rmsnorm,
                 lib.mvllm_last_error)))
+        self._rolling = None if self._host is None else self._host.rolling_entries(*(
+            ctypes.cast(f, ctypes.c_void_p).value for f in (
+                lib.mvllm_paged_window_attention_plan, lib.mvllm_paged_window_attention,
+                lib.mvllm_rope_kv_write, lib.mvllm_last_error)))
 
     # The ops below in native code (csrc/host/host.cpp): the result, or None where the call
     # is not one that it serves as it stands and the Python body has to look at it. Their
@@ -567,6 +571,14 @@ class HipExtension:
         if self._host is None or self._recording is not None:
             return None
         return self._host.paged_decode_qk_norm_rope(self._entries, self._workspaces, *args)
+
+    def try_paged_window_attention(self, *args):
+        if self._host is None or self._recording is not None:
+            return None
+        return self._host.paged_window_attention(self._rolling, self._workspaces, *args)
+
+    def try_rope_kv_write(self, *args):  # (takes no workspace)
+        return None if self._host is None else self._host.rope_kv_write(self._rolling, *args)
 
     def workspace(self, device: torch.device, nbytes: int) -> torch.Tensor:
         """The kernels' workspace of (device, current stream), grown on demand (paged and

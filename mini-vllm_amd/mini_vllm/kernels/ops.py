@@ -696,13 +696,19 @@ def paged_window_attention(
         raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    if _use_kernel("paged_attention", use_cuda, q) and _served(
-            "paged_window_attention", _kernel_can_page(q, key_pool, value_pool, block_tables,
-                                                       (cu_seqlens_q, context_lens, seq_lens))):
-        return load_extension().paged_window_attention(
+    if _use_kernel("paged_attention", use_cuda, q):
+        ext = load_extension()
+        served = ext.try_paged_window_attention(
             q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens, seq_lens,
-            int(max_query_len), int(max_context_len), int(window), int(sinks), scale, k_scale,
-            v_scale)
+            max_query_len, max_context_len, window, sinks, scale, k_scale, v_scale)
+        if served is not None:
+            return served
+        if _served("paged_window_attention", _kernel_can_page(
+                q, key_pool, value_pool, block_tables, (cu_seqlens_q, context_lens, seq_lens))):
+            return ext.paged_window_attention(
+                q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens, seq_lens,
+                int(max_query_len), int(max_context_len), int(window), int(sinks), scale, k_scale,
+                v_scale)
     return torch_path.paged_window_attention_gathered(
         q, key_pool, value_pool, block_tables, cu_seqlens_q, context_lens, window, sinks, scale,
         k_scale=k_scale, v_scale=v_scale)
@@ -765,10 +771,16 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     neither). A pool of q's dtype gets the bits of :func:`rope` then :func:`kv_write`; a
     ``float8_e4m3fn`` one is quantised by the same policy from the float32 rotation, not rounded
     to k's dtype between. q, k and v may be column views of one projection's output."""
-    if _use_kernel("kv_write", use_cuda, q) and _served("rope_kv_write", _rope_kv_write_reason(
-            q, k, v, positions, cos, sin, key_pool, value_pool, slot_mapping)):
-        return load_extension().rope_kv_write(q, k, v, positions, cos, sin, key_pool, value_pool,
-                                              slot_mapping, k_scale, v_scale)
+    if _use_kernel("kv_write", use_cuda, q):
+        ext = load_extension()
+        served = ext.try_rope_kv_write(q, k, v, positions, cos, sin, key_pool, value_pool,
+                                       slot_mapping, k_scale, v_scale)
+        if served is not None:
+            return served
+        if _served("rope_kv_write", _rope_kv_write_reason(q, k, v, positions, cos, sin, key_pool,
+                                                          value_pool, slot_mapping)):
+            return ext.rope_kv_write(q, k, v, positions, cos, sin, key_pool, value_pool,
+                                     slot_mapping, k_scale, v_scale)
     return torch_path.rope_kv_write(q, k, v, positions, cos, sin, key_pool, value_pool,
                                     slot_mapping, k_scale=k_scale, v_scale=v_scale)
 

@@ -192,6 +192,21 @@ def test_captured_and_replayed_on_another_stream(device, pairs):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype,kv_dtype", [TYPES[0], TYPES[2], TYPES[4]])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_freed_page_that_is_seen_reads_within_the_pool(device, d, dtype, kv_dtype):
+    """A window larger than the one pages were freed for: the sequences it makes no difference to
+    are right, the others' rows are whatever the pool's last page gives."""
+    b = rolling_batch(MIXED, 40, 5, dtype=dtype, kv_dtype=kv_dtype, hq=4, hk=2, d=d)
+    out = call({**b, "window": 4000}, device).double().cpu()
+    want, tolerance = expected(b)
+    cu = b["cu_seqlens_q"].tolist()
+    for s, (held, new) in enumerate(MIXED):
+        if held <= 40:
+            rows = slice(cu[s], cu[s + 1])
+            assert ((out[rows] - want[rows]).abs() <= tolerance[rows]).all()
+
+
 def test_two_calls_give_the_same_bits(device):
     b = on(rolling_batch(DECODES + CHUNKS, 200, 4, dtype=torch.bfloat16, kv_dtype=torch.float8_e4m3fn), device)
     first = call(b, device).clone()
