@@ -81,10 +81,11 @@ struct Options {
   int prefill_piece_pct = mvllm::kSplitDefaultPct;
 };
 
-int read_options(const mvllm_plan_options* o, Options& out) {
+int read_options(const mvllm_plan_options* o, Options& out, bool windowed = false) {
   out = Options{};
   if (o == nullptr) return MVLLM_OK;
-  if (o->decode_schedule < 0 || o->decode_schedule > MVLLM_DECODE_GRID ||
+  if (o->decode_schedule < 0 || (o->decode_schedule > MVLLM_DECODE_GRID &&
+                                 !(windowed && o->decode_schedule == MVLLM_DECODE_DIRECT)) ||
       o->prefill_schedule < 0 || o->prefill_schedule > 2 || o->prefill_staging < 0 ||
       o->prefill_staging > 1 || o->decode_wgs_per_cu < 0 || o->decode_waves_per_cu < 0 ||
       o->decode_split_tokens < 0 || o->prefill_wgs_per_cu < 0 || o->prefill_share_tiles < 0 ||
@@ -185,7 +186,7 @@ uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk,
                  int32_t d, int32_t block_size, int32_t max_q, int32_t max_ctx, int32_t q_dtype,
-                 int32_t kv_dtype, const Options& o);
+                 int32_t kv_dtype, const Options& o, bool windowed);
 
 // Whether the pair prefill kernel serves these prefill rows (but for the sign of the
 // scale, which only the launch knows): D = 128, GQA pairs, pages of >= 16 keys, 16-bit
@@ -401,7 +402,8 @@ Plan make_plan(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int
   Plan plan{};
   // A single query's keys: its context, or its windowed list.
   const int32_t keys = win.window > 0 ? mvllm::window_keys(max_ctx, win.window, win.sinks) : max_ctx;
-  plan_decode(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, keys, q_dtype, kv_dtype, o);
+  plan_decode(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, keys, q_dtype, kv_dtype, o,
+              win.window > 0);
   plan_prefill(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, max_ctx, q_dtype, kv_dtype,
                o, win);
   if (plan.pub.prefill_mfma && pair_prefill(hq, hk, d, block_size, q_dtype, kv_dtype, o)) {
@@ -411,9 +413,24 @@ Plan make_plan(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int
   return plan;
 }
 
+// Windowed decode: the direct schedule or the stream, for lists of at most `keys` entries, from what
+// each was measured to take (us a call): direct 4.5 + a list at 34 bytes a ns (30 over fp8), the
+// stream 10 + all lists at 6.2 TB/s, while a CU has one list at most. Direct and stream, bf16, 8 kv
+// heads: one sequence of 64 keys 4.8 and 9.5, of 512 10.1 and 11.1, of 1024 17 and 11.5; 16 of 1024 19.2
+// and 19.2, of 2048 33 and 29; 28 of 1024 23 and 28.
+//   Past that both run at the memory's rate and direct saves the second launch (64 of 1024 46 and
+// 49, 256 of 1024 169 and 174), but for fp8: rows of 128 bytes apart are read at 5 TB/s, the stream's
+// whole tokens at 6 (64 of 4096 112 and 96, 256 of 1024 109 and 97), so only short lists of not
+// too many (64 of 1024 31 and 32, 128 of 512 31 and 33).
+bool direct_decode(int64_t lists, int64_t keys, int64_t row_bytes, bool fp8, int cus) {
+  if (lists > cus) return !fp8 || (lists <= 4 * cus && keys <= 1024);
+  const double list = 2.0 * static_cast<double>(keys * row_bytes);
+  return 4.5e3 + list / (fp8 ? 30 : 34) <= 10e3 + list * static_cast<double>(lists) / 6200;
+}
+
 void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk,
                  int32_t d, int32_t block_size, int32_t max_q, int32_t max_ctx, int32_t q_dtype,
-                 int32_t kv_dtype, const Options& o) {
+                 int32_t kv_dtype, const Options& o, bool windowed) {
   const bool has_prefill = max_q > 1;
   const bool mfma =
       has_prefill && mvllm::paged_prefill_supported(q_dtype, kv_dtype, d, hq, hk, block_size);
@@ -428,6 +445,14 @@ void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, i
     plan.pub.decode_mode = MVLLM_DECODE_BY_ROW;
   } else if (all_prefill || num_seqs == 0) {
     plan.pub.decode_mode = MVLLM_DECODE_NONE;
+  } else if (windowed && num_seqs < 65536 &&
+             (o.decode_schedule == MVLLM_DECODE_DIRECT ||
+              (o.decode_schedule == 0 &&
+               direct_decode(num_seqs * units, max_ctx, static_cast<int64_t>(d) * element_bytes(kv_dtype),
+                             kv_dtype == mvllm::kFP8E4M3, device_cus())))) {
+    plan.pub.decode_mode = MVLLM_DECODE_DIRECT;
+    plan.pub.decode_workgroups = static_cast<int32_t>(num_seqs * units);
+    return;
   } else if (num_seqs <= mvllm::kMaxStreamSeqs && units <= 8 &&
              static_cast<int64_t>(num_seqs) * max_ctx < (int64_t{1} << 31) &&
              o.decode_schedule != MVLLM_DECODE_GRID) {
@@ -494,6 +519,7 @@ std::atomic<int64_t> g_split_whole_capturing{0};  // cut grid launches run whole
 int launch_planned(const Plan& plan, mvllm::PagedParams& p, void* workspace, int32_t q_dtype,
                    int32_t kv_dtype, int32_t head_dim, int32_t max_query_len, hipStream_t s,
                    const char* name) {
+  p.direct = plan.pub.decode_mode == MVLLM_DECODE_DIRECT ? 1 : 0;
   p.stream_wgs = plan.pub.decode_mode == MVLLM_DECODE_STREAM ? plan.pub.decode_workgroups : 0;
   p.stream_min_keys = mvllm::decode_min_share_keys(element_bytes(kv_dtype), head_dim);
   p.split_tokens = plan.pub.split_tokens > 0 ? plan.pub.split_tokens : mvllm::kMaxSplitTokens;
@@ -759,7 +785,7 @@ int paged_attention_entry(const char* name, void* out, const void* q, const void
                              block_size, max_query_len, max_context_len, q_dtype, kv_dtype);
   if (rc != MVLLM_OK) return rc;
   Options o;
-  rc = read_options(options, o);
+  rc = read_options(options, o, win.window > 0);
   if (rc != MVLLM_OK) return rc;
   if (static_scratch) o.scratch_bytes = workspace_bytes;
   if (num_tokens == 0 || num_seqs == 0) return MVLLM_OK;
@@ -926,7 +952,7 @@ int mvllm_paged_window_attention_plan(int32_t num_tokens, int32_t num_seqs, int3
                              block_size, max_query_len, max_context_len, q_dtype, kv_dtype);
   if (rc != MVLLM_OK) return rc;
   Options o;
-  rc = read_options(options, o);
+  rc = read_options(options, o, true);
   if (rc != MVLLM_OK) return rc;
   Window win;
   rc = read_window(window, sinks, max_context_len, win);

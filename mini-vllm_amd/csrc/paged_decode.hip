@@ -921,6 +921,78 @@ __global__ __launch_bounds__(256) void paged_decode_grid_merge_kernel(const Page
   }
 }
 
+// ------------------------------------------------------------ direct schedule
+
+// Windowed decode by a workgroup per (sequence, kv head, chunk of its query heads): its waves take
+// equal runs of the sequence's list and meet in LDS, so there is one launch, and no partials or
+// prefix sums in memory. A window bounds every list, so a workgroup per list is balanced enough, where
+// full contexts need the stream's equal shares. The stream's second launch and its chain of
+// partials cost 5 us whatever the batch: 28 lists of 128 keys 11.9 -> 6.7 us, of 700 over fp8 24 ->
+// 14, 64 of 1028 48.9 -> 46.1. What bounds it, besides memory: a CU takes in about 35 GB/s (30 over
+// fp8, whose rows are 128 bytes), so few lists that are long stay with the stream (one of 1028 17.0
+// against 11.5). 16 waves instead of 8 measured the same.
+template <typename TQ, typename TKV, int D, int GC>
+__global__ __launch_bounds__(kMaxDecodeWaves * kWave) void paged_decode_direct_kernel(const PagedParams p) {
+  using K = Decode<TQ, TKV, D, GC>;
+  constexpr int kWaves = kMaxDecodeWaves;
+  __shared__ __align__(16) float s_o[kWaves][GC][D];
+  __shared__ float s_m[kWaves][GC], s_l[kWaves][GC];
+  const int seq = blockIdx.y;
+  if (sload(p.seq_lens + seq) != 1) return;  // a prefill chunk: the prefill kernel has it
+  const int context = max(sload(p.context_lens + seq), 0);
+  const int row = sload(p.cu_seqlens_q + seq);
+  const int entries = window_keys(context, p.window, p.sinks);
+  int kvh, h0;
+  if (!wave_unit<GC>(p, blockIdx.x, kvh, h0)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int g = lane / K::R, r = lane % K::R;
+  constexpr int kStep = K::RG * kUnroll;
+  const int per = ((entries + kWaves - 1) / kWaves + kStep - 1) / kStep * kStep;
+  const int sb = min(wave * per, entries), se = min(sb + per, entries);
+  typename K::State st;
+  K::init(st);
+  if (sb < se) {
+    typename K::Q qf[GC];
+    K::load_queries(p, row, h0, r, qf);
+    const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks;
+    K::stream_window(p, table, WindowKeys{p.sinks, context - entries}, kvh, sb, se, g, r, qf,
+                     p.scale * kLog2e, st);
+    K::merge_row_groups(st);
+  }
+  if (g == 0) {
+#pragma unroll
+    for (int h = 0; h < GC; ++h) {
+#pragma unroll
+      for (int e = 0; e < K::E; e += 4) {
+        *reinterpret_cast<f32x4*>(&s_o[wave][h][r * K::E + e]) =
+            f32x4{st.acc[h][e], st.acc[h][e + 1], st.acc[h][e + 2], st.acc[h][e + 3]};
+      }
+      if (r == 0) {
+        s_m[wave][h] = st.m[h];
+        s_l[wave][h] = st.l[h];
+      }
+    }
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < GC * D; j += kWaves * kWave) {
+    const int h = j / D, d = j % D;
+    float m = s_m[0][h];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][h]);
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float a = fast_exp2(s_m[w][h] - mu);
+      l = fmaf(s_l[w][h], a, l);
+      o = fmaf(s_o[w][h][d], a, o);
+    }
+    // (no key at all: l = 0, a row of zeros)
+    Elem<TQ>::store(p.out, (static_cast<int64_t>(row) * p.hq + h0 + h) * D + d,
+                    l > 0.0f ? o * (1.0f / l) : 0.0f);
+  }
+}
+
 // ------------------------------------------------------------------ dispatch
 
 namespace {
@@ -955,6 +1027,13 @@ hipError_t launch_decode_g(const PagedParams& p, hipStream_t stream) {
   const int units = p.hk * (p.hq / p.hk / GC);
   const int waves = decode_waves(p, GC);
   constexpr int kHeadsPerMergeBlock = 4;
+  if constexpr (kWindow) {
+    if (p.direct != 0) {
+      paged_decode_direct_kernel<TQ, TKV, D, GC>
+          <<<dim3(units, p.num_seqs), kMaxDecodeWaves * kWave, 0, stream>>>(p);
+      return hipGetLastError();
+    }
+  }
   if (p.stream_wgs > 0) {
     if (units > 8) return hipErrorInvalidValue;  // planner keeps stream mode to <= 8 units
     paged_decode_stream_kernel<TQ, TKV, D, GC, false, kWindow>

@@ -95,11 +95,29 @@ def test_plan_refusals(lib):
         plan(lib, head_dim=96)
 
 
+def test_decode_schedules(lib):
+    """A workgroup per list where that is the faster one, without a workspace; the stream for few
+    long lists and for many over fp8; a forced one; none of it for calls without a window."""
+    def mode(n, window, **more):
+        return plan(lib, window=window, num_tokens=n, num_seqs=n, max_context_len=30000, **more)["decode_mode"]
+    fp8 = {"kv_dtype": torch.float8_e4m3fn}
+    assert mode(1, 128) == mode(28, 700) == mode(28, 700, **fp8) == mode(300, 4000) == "direct"
+    assert mode(1, 4000) == mode(4, 4000, **fp8) == mode(256, 4000, **fp8) == mode(300, 100, **fp8) == "stream"
+    assert mode(4200, 100) == "direct" and mode(4200, 100, **fp8) == "grid"
+    direct = plan(lib, window=128, options={"decode_schedule": 4})
+    assert direct["decode_mode"] == "direct" and direct["workspace_bytes"] == 0
+    assert direct["decode_workgroups"] == 4 * 8
+    with pytest.raises(RuntimeError, match="out of range"):
+        lib.paged_attention_plan(4, 4, 16, 8, 128, 16, 1, 100, torch.bfloat16, torch.bfloat16,
+                                 {"decode_schedule": 4})
+
+
 def test_a_plan_goes_by_the_window_not_the_context(lib):
     # the fewest keys of a share at this type are 16: no more workgroups than shares of the window
-    assert plan(lib, window=128, sinks=4, num_tokens=1, num_seqs=1,
-                max_context_len=2**29)["decode_workgroups"] == 9
-    assert (plan(lib, window=2**31 - 1, sinks=2**31 - 1)["decode_workgroups"]
+    stream = {"decode_schedule": 1}
+    assert plan(lib, window=128, sinks=4, num_tokens=1, num_seqs=1, max_context_len=2**29,
+                options=stream)["decode_workgroups"] == 9
+    assert (plan(lib, window=2**31 - 1, sinks=2**31 - 1, options=stream)["decode_workgroups"]
             == lib.paged_attention_plan(4, 4, 16, 8, 128, 16, 1, 4096, torch.bfloat16,
                                         torch.bfloat16)["decode_workgroups"])
     by_row = plan(lib, num_tokens=100, num_seqs=1, max_query_len=100, q_dtype=torch.float32,

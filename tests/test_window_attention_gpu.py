@@ -69,13 +69,29 @@ def test_fp8_scales_that_are_no_powers_of_two(device, dtype):
     assert_close(call(b, device), b)
 
 
-@pytest.mark.parametrize("schedule", ["stream", "grid"])
+SCHEDULES = {"stream": 1, "grid": 2, "direct": 4}
+
+
+@pytest.mark.parametrize("dtype,kv_dtype", TYPES)
+@pytest.mark.parametrize("schedule", SCHEDULES)
+@pytest.mark.parametrize("hq,hk,d", [(16, 8, 128), (4, 1, 64), (3, 3, 32), (6, 1, 256)])
+def test_decode_schedules(device, extension, schedule, hq, hk, d, dtype, kv_dtype):
+    b = rolling_batch(DECODES + [(0, 1), (40, 0)], 70, 9, dtype=dtype, kv_dtype=kv_dtype, hq=hq, hk=hk, d=d)
+    args = on(b, device)
+    got = extension.paged_window_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], 1, b["max_context_len"], 70, 9, b["scale"],
+        args["k_scale"], args["v_scale"], plan_options={"decode_schedule": SCHEDULES[schedule]})
+    assert_close(got, b, schedule)
+
+
+@pytest.mark.parametrize("schedule", SCHEDULES)
 @pytest.mark.parametrize("n", [65, 300])
 def test_many_sequences(device, extension, n, schedule):
     """More sequences than a wave has lanes, and rows without keys among them."""
     pairs = [(37 * i % 301, 1) for i in range(n)]
     b = rolling_batch(pairs, 100, 4, dtype=torch.bfloat16, hq=4, hk=2)
-    options = {"decode_schedule": 1 if schedule == "stream" else 2, "decode_split_tokens": 64}
+    options = {"decode_schedule": SCHEDULES[schedule], "decode_split_tokens": 64}
     args = on(b, device)
     got = extension.paged_window_attention(
         args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
