@@ -198,18 +198,29 @@ __device__ __forceinline__ float finite_max(float m, const float (&x)[E]) {
   return m;
 }
 
-// Workgroups [0, kv_wgs): window (blockIdx / hk) of tokens_per_wg tokens, kv head blockIdx % hk: the
-// runs that start in the window, one after another. The rest: q, G heads a thread.
+// Every `every`th workgroup while there are q_wgs: q, G heads a thread. The others: a window of tokens
+// and a kv head, kRows tokens at a time, a row of threads each (K's pieces, then V's).
+//   A window's workgroup writes the runs that start in it, all at once: the rows from its first start
+// to the end of its last run, which may lie in the next window. Slots and positions are loaded once,
+// a lane each, and handed round from there; runs are stretches of two bit masks; a run's maxima meet
+// in LDS (the order of a maximum does not matter). So a run's rows, angles and old scale are
+// requested one round trip after the launch, and 16 single tokens take as long as a page of 16.
+// One run after another, each finding its slots, length, positions and angles in turn, and q's
+// workgroups last: 8704 tokens in eight chunks 37.7 us, now 31.4 (4.3 TB/s); 128 tokens 10.3, now 6.5;
+// 2048 single tokens 44.9, now 11.9; 64 level at 4.4.
 template <typename T, typename TPos, int D, int G>
-__global__ __launch_bounds__(256) void rope_write_fp8_kernel(const RopeWriteParams p, int kv_wgs,
-                                                             int tokens_per_wg, uint32_t q_threads) {
+__global__ __launch_bounds__(256) void rope_write_fp8_kernel(const RopeWriteParams p, int every,
+                                                             int q_wgs, uint32_t q_threads) {
   constexpr int kBytes = Elem<T>::kBytes;
-  constexpr int kPieces = D / 2 / E;      // threads of a head vector
+  constexpr int kPieces = D / 2 / E;        // threads of a head vector
   constexpr int kRowThreads = 2 * kPieces;  // of a row: K's, then V's
+  constexpr int kRows = 256 / kRowThreads;  // of a pass, and tokens of a window
   constexpr int64_t kRow = static_cast<int64_t>(D) * kBytes;
-  static_assert(kRowThreads <= kWave, "head dim");
-  if (static_cast<int>(blockIdx.x) >= kv_wgs) {
-    const uint32_t index = (blockIdx.x - kv_wgs) * blockDim.x + threadIdx.x;
+  static_assert(kRows <= kWave, "a window's tokens are held a lane each");
+  const int bid = static_cast<int>(blockIdx.x);
+  const int q_before = min(bid / every, q_wgs);
+  if (q_before < q_wgs && bid % every == every - 1) {
+    const uint32_t index = static_cast<uint32_t>(q_before) * 256 + threadIdx.x;
     if (index >= q_threads) return;
     const uint32_t per_token = static_cast<uint32_t>(p.hq / G) * kPieces;
     const int token = static_cast<int>(index / per_token);
@@ -224,108 +235,154 @@ __global__ __launch_bounds__(256) void rope_write_fp8_kernel(const RopeWritePara
                      position_of<TPos>(p, token), D, piece);
     return;
   }
-  __shared__ float s_max[4][2];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int waves = blockDim.x / kWave;
-  const int head = static_cast<int>(blockIdx.x) % p.hk;
-  const int first = static_cast<int>(blockIdx.x) / p.hk * tokens_per_wg;
-  const int rows = blockDim.x / kRowThreads;  // of a pass
+  __shared__ uint32_t s_max[kRows][2];  // of the window's runs, the bits of a float >= 0
+  __shared__ float s_old[kRows][2];     // their pages' scales before
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int head = (bid - q_before) % p.hk;
+  const int first = (bid - q_before) / p.hk * kRows;
   const int my_row = tid / kRowThreads;
   const bool is_v = tid % kRowThreads >= kPieces;
   const int piece = tid % kPieces;
 
-  // A token starts a run when its slot is in the pool and does not continue the slot of the token
-  // before on the same page.
-  uint64_t starts;
-  {
-    const int t = first + lane;
-    bool start = false;
-    if (lane < tokens_per_wg && t < p.tokens) {
-      const int slot = p.slots[t];
-      const int prev = t > 0 ? p.slots[t - 1] : -1;
-      start = slot >= 0 && (slot >> p.block_shift) < p.num_blocks &&
-              !(prev >= 0 && prev + 1 == slot && (prev >> p.block_shift) == (slot >> p.block_shift));
+  // Lane i: token first + i. It starts a run when its slot is in the pool and does not continue the
+  // slot of the token before on the same page.
+  const int mine = min(first + lane, p.tokens - 1);
+  const int my_slot = p.slots[mine];
+  const TPos my_position = static_cast<const TPos*>(p.positions)[mine];
+  const int slot_before = first > 0 ? p.slots[first - 1] : -1;
+  const int up = __shfl_up(my_slot, 1, kWave);
+  const int prev = lane > 0 ? up : slot_before;
+  const bool live = first + lane < p.tokens && my_slot >= 0 && (my_slot >> p.block_shift) < p.num_blocks;
+  const bool goes_on = live && prev >= 0 && prev + 1 == my_slot &&
+                       (prev >> p.block_shift) == (my_slot >> p.block_shift);
+  const uint64_t window = kRows == kWave ? ~uint64_t{0} : (uint64_t{1} << (kRows % kWave)) - 1;
+  const uint64_t on = __builtin_amdgcn_ballot_w64(goes_on);
+  const uint64_t starts = __builtin_amdgcn_ballot_w64(live && !goes_on) & window;
+  if (starts == 0) return;  // the whole workgroup
+  const int i0 = __builtin_ctzll(starts);
+  // The last run's rows behind the window: lanes, then tokens past the lanes.
+  int end = kRows;  // (a lane, or past them)
+  while (end < kWave && (on >> (end % kWave) & 1)) ++end;
+  if (end == kWave) {
+    const int last = 63 - __builtin_clzll(starts);
+    if (kRows < kWave || (on >> 63 & 1) || last == 63) {
+      const int slot_last = __builtin_amdgcn_readlane(my_slot, last);
+      const int room = (1 << p.block_shift) - (slot_last & ((1 << p.block_shift) - 1));
+      for (bool more = true; more; ) {
+        const int i = end + lane;
+        const bool same = i - last < room && first + i < p.tokens && p.slots[first + i] == slot_last + i - last;
+        const uint64_t not_same = __builtin_amdgcn_ballot_w64(!same);
+        end += not_same != 0 ? __builtin_ctzll(not_same) : kWave;
+        more = not_same == 0;
+      }
     }
-    starts = __builtin_amdgcn_ballot_w64(start);
   }
-  while (starts != 0) {
-    const int t0 = first + __builtin_ctzll(starts);
-    starts &= starts - 1;
-    const int slot0 = __builtin_amdgcn_readfirstlane(p.slots[t0]);
-    const int page = slot0 >> p.block_shift;
-    const int off0 = slot0 & ((1 << p.block_shift) - 1);
-    const int limit = min((1 << p.block_shift) - off0, p.tokens - t0);
-    int len = limit;
-    for (int base = 1; base < limit; base += kWave) {
-      const int i = base + lane;
-      const uint64_t stop = __builtin_amdgcn_ballot_w64(i < limit && p.slots[t0 + i] != slot0 + i);
-      if (stop != 0) {
-        len = base + __builtin_ctzll(stop);
-        break;
-      }
-    }
-    float* scale_at = (is_v ? p.v_scales : p.k_scales) + static_cast<int64_t>(page) * p.hk + head;
-    const float old = off0 > 0 ? *scale_at : 0.0f;
-    uint8_t* pool = static_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) +
-                    ((static_cast<int64_t>(page) << p.block_shift) * p.hk + head) * D + piece * E;
-    const int64_t pool_row = static_cast<int64_t>(p.hk) * D;
+  const int passes = (end - i0 + kRows - 1) / kRows;
 
-    float x[E], y[E];
-    auto take = [&](int i) {  // row i of the run, turned
-      const int t = t0 + i;
-      const char* src = static_cast<const char*>(is_v ? p.v : p.k) +
-                        (t * (is_v ? p.v_stride : p.k_stride) * kBytes + head * kRow + piece * E * kBytes);
-      Piece<T> lo, hi;
-      lo.load(src);
-      hi.load(src + kRow / 2);
-      if (!is_v) {
-        Angles a;
-        a.load(p, position_of<TPos>(p, t), D, piece);
-        lo.unpack(x);
-        hi.unpack(y);
-        a.turn(x, y);
-      } else {
-        lo.unpack(x);
-        hi.unpack(y);
-      }
-    };
+  // This thread's row of a pass: its run, the run's first slot, and the row's token.
+  int token = 0, run = 0, run_slot = 0, in_run = 0, run_rows = 0;
+  int64_t position = 0;
+  bool row = false;
+  auto find = [&](int pass) __attribute__((always_inline)) {
+    const int i = i0 + pass * kRows + my_row;
+    const int at = min(i, kWave - 1);
+    const uint64_t before = starts & (at == kWave - 1 ? ~uint64_t{0} : (uint64_t{2} << at) - 1);
+    const int start = 63 - __builtin_clzll(before);  // (i0 is among them)
+    run = __builtin_popcountll(before) - 1;
+    row = i < end && (i >= kWave || ((starts | on) >> at & 1));
+    token = first + i;
+    in_run = i - start;
+    const uint64_t stops = ~on & (start == kWave - 1 ? 0 : ~uint64_t{0} << (start + 1));
+    const int stop = stops != 0 ? min(__builtin_ctzll(stops), end) : end;
+    run_rows = stop - start;
+    run_slot = __shfl(my_slot, start, kWave);
+    const int low = __shfl(static_cast<int>(my_position), at, kWave);
+    position = low;
+    if constexpr (sizeof(TPos) == 8) {
+      const int high = __shfl(static_cast<int>(static_cast<int64_t>(my_position) >> 32), at, kWave);
+      position = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(high)) << 32 |
+                                      static_cast<uint32_t>(low));
+    }
+    if (row && i >= kWave) position = position_of<TPos>(p, token);
+  };
+  float x[E], y[E];
+  auto take = [&]() __attribute__((always_inline)) {  // the row, turned
+    const char* src = static_cast<const char*>(is_v ? p.v : p.k) +
+                      (token * (is_v ? p.v_stride : p.k_stride) * kBytes + head * kRow + piece * E * kBytes);
+    Piece<T> lo, hi;
+    lo.load(src);
+    hi.load(src + kRow / 2);
+    Angles a;
+    if (!is_v) a.load(p, position, D, piece);
+    lo.unpack(x);
+    hi.unpack(y);
+    if (!is_v) a.turn(x, y);
+  };
+
+  auto scale_at = [&]() __attribute__((always_inline)) -> float* {
+    return (is_v ? p.v_scales : p.k_scales) +
+           (static_cast<int64_t>(run_slot >> p.block_shift) * p.hk + head);
+  };
+
+  for (int i = tid; i < 2 * kRows; i += 256) s_max[i / 2][i % 2] = 0;
+  __syncthreads();
+  for (int pass = 0; pass < passes; ++pass) {
+    find(pass);
     float most = 0.0f;
-    for (int i = my_row; i < len; i += rows) {
-      take(i);
-      most = finite_max(finite_max(most, x), y);
+    if (row) {
+      if (in_run == 0 && piece == 0) {
+        s_old[run][is_v] = (run_slot & ((1 << p.block_shift) - 1)) != 0 ? *scale_at() : 0.0f;
+      }
+      take();
+      most = finite_max(finite_max(0.0f, x), y);
     }
     most = group_max<kPieces>(most);
-#pragma unroll
-    for (int off = kRowThreads; off < kWave; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, kWave));
-    if (waves > 1) {
-      if (lane < kRowThreads && piece == 0) s_max[wave][is_v] = most;
-      __syncthreads();
-      for (int w = 0; w < waves; ++w) most = fmaxf(most, s_max[w][is_v]);
-      __syncthreads();
+    if (row && piece == 0) atomicMax(&s_max[run][is_v], __float_as_uint(most));
+  }
+  __syncthreads();
+  for (int pass = 0; pass < passes; ++pass) {
+    if (passes > 1) {  // (else the row is held still)
+      find(pass);
+      if (row) take();
     }
-    const float scale = fmaxf(old, pow2_at_least(most / 448.0f));
+    if (!row) continue;
+    const float old = s_old[run][is_v];
+    const float scale = fmaxf(old, pow2_at_least(__uint_as_float(s_max[run][is_v]) / 448.0f));
     const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;  // exact: a power of two
-
-    if (old > 0.0f && scale > old) {  // the page's earlier rows under the grown scale
-      for (int r = my_row; r < off0; r += rows) {
+    const int64_t pool_row = static_cast<int64_t>(p.hk) * D;
+    const int off0 = run_slot & ((1 << p.block_shift) - 1);
+    uint8_t* pool = static_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) +
+                    (static_cast<int64_t>(run_slot - off0) * p.hk + head) * D + piece * E;
+    if (old > 0.0f && scale > old) {  // the page's earlier rows, shared out among the run's
+      constexpr int kAhead = 4;
+      for (int r0 = in_run; r0 < off0; r0 += kAhead * run_rows) {
+        u32x2 w[kAhead][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint8_t* at = pool + r * pool_row + h * (D / 2);
-          const u32x2 w = *reinterpret_cast<const u32x2*>(at);
-          float v[E];
+        for (int u = 0; u < kAhead; ++u) {
+          const int r = r0 + u * run_rows < off0 ? r0 + u * run_rows : r0;
 #pragma unroll
-          for (int b = 0; b < E; ++b) v[b] = __fmul_rn(fp8e4m3_to_f32((w[b / 4] >> (8 * (b % 4))) & 0xffu), old);
-          *reinterpret_cast<u32x2*>(at) = encode8(v, inv);
+          for (int h = 0; h < 2; ++h) w[u][h] = *reinterpret_cast<const u32x2*>(pool + r * pool_row + h * (D / 2));
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int r = r0 + u * run_rows;
+          if (r >= off0) continue;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[E];
+#pragma unroll
+            for (int b = 0; b < E; ++b) {
+              v[b] = __fmul_rn(fp8e4m3_to_f32((w[u][h][b / 4] >> (8 * (b % 4))) & 0xffu), old);
+            }
+            *reinterpret_cast<u32x2*>(pool + r * pool_row + h * (D / 2)) = encode8(v, inv);
+          }
         }
       }
     }
-    for (int i = my_row; i < len; i += rows) {
-      if (len > rows) take(i);  // (else still held)
-      uint8_t* at = pool + (off0 + i) * pool_row;
-      *reinterpret_cast<u32x2*>(at) = encode8(x, inv);
-      *reinterpret_cast<u32x2*>(at + D / 2) = encode8(y, inv);
-    }
-    if (my_row == 0 && piece == 0) *scale_at = scale;
+    if (in_run == 0 && piece == 0) *scale_at() = scale;
+    uint8_t* at = pool + (off0 + in_run) * pool_row;
+    *reinterpret_cast<u32x2*>(at) = encode8(x, inv);
+    *reinterpret_cast<u32x2*>(at + D / 2) = encode8(y, inv);
   }
 }
 
@@ -362,19 +419,17 @@ hipError_t launch_same(const RopeWriteParams& p, int dim, hipStream_t stream) {
 
 template <typename T, typename TPos, int D>
 hipError_t launch_fp8(const RopeWriteParams& p, hipStream_t stream) {
-  constexpr int kPieces = D / 2 / E;
-  const bool large = p.tokens >= 2048;
-  const int tokens_per_wg = large ? 16 : 1;
-  const unsigned bs = large ? 256 : 64;
-  const int64_t kv_wgs = (p.tokens + tokens_per_wg - 1) / tokens_per_wg * static_cast<int64_t>(p.hk);
+  constexpr int kPieces = D / 2 / E, kRows = 256 / (2 * kPieces);
+  const int64_t kv_wgs = (p.tokens + kRows - 1) / kRows * static_cast<int64_t>(p.hk);
   const int64_t q_all = static_cast<int64_t>(p.tokens) * p.hq * kPieces;
   const int g = heads_per_thread(q_all, p.hq, p.hq);
   const int64_t q_threads = q_all / g;
-  const int64_t grid = kv_wgs + (q_threads + bs - 1) / bs;
+  const int64_t q_wgs = (q_threads + 255) / 256, grid = kv_wgs + q_wgs;
   if (q_threads >= int64_t{1} << 31 || grid >= int64_t{1} << 31) return hipErrorInvalidValue;
-#define MVLLM_ROPE_WRITE(G)                                                           \
-  rope_write_fp8_kernel<T, TPos, D, G><<<static_cast<unsigned>(grid), bs, 0, stream>>>( \
-      p, static_cast<int>(kv_wgs), tokens_per_wg, static_cast<uint32_t>(q_threads))
+  const int every = static_cast<int>(grid / q_wgs);  // (>= 1: every q_wgs-th position is in the grid)
+#define MVLLM_ROPE_WRITE(G)                                                            \
+  rope_write_fp8_kernel<T, TPos, D, G><<<static_cast<unsigned>(grid), 256, 0, stream>>>( \
+      p, every, static_cast<int>(q_wgs), static_cast<uint32_t>(q_threads))
   if (g == 4) MVLLM_ROPE_WRITE(4);
   else if (g == 2) MVLLM_ROPE_WRITE(2);
   else MVLLM_ROPE_WRITE(1);
