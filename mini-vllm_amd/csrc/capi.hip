@@ -433,7 +433,8 @@ void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, i
                  int32_t kv_dtype, const Options& o, bool windowed) {
   const bool has_prefill = max_q > 1;
   const bool mfma =
-      has_prefill && mvllm::paged_prefill_supported(q_dtype, kv_dtype, d, hq, hk, block_size);
+      has_prefill && (windowed ? mvllm::window_prefill_supported(q_dtype, kv_dtype, d)
+                               : mvllm::paged_prefill_supported(q_dtype, kv_dtype, d, hq, hk, block_size));
   // Query lengths are at most max_q and sum to num_tokens, so num_tokens ==
   // num_seqs * max_q (with max_q > 1) means every sequence is a prefill chunk.
   const bool all_prefill =

@@ -204,7 +204,8 @@ struct PagedParams {
   int pf_share_tiles;       // stream prefill: fewest key tiles per share; pair prefill:
                             // fewest key tiles per piece
   int pf_register_staging;  // 1: the register-staged prefill kernel even where the
-                            // direct-to-LDS one serves (a plan option, for measurement)
+                            // direct-to-LDS one serves (a plan option, for measurement);
+                            // windowed: the general kernel even where the pair one serves
   int pf_tile;        // pair prefill: query positions of an item, 64 or 128
   int pf_pieces;      // pair prefill: 0 the (column, sequence, query tile) grid; else a 1-D grid
                       // of pf_ranks x columns by the schedule, items in at most this
@@ -287,6 +288,11 @@ hipError_t launch_paged_decode_fresh(const PagedParams& p, const FreshParams& f,
 
 hipError_t launch_paged_prefill(const PagedParams& p, int q_dtype, int kv_dtype, int head_dim,
                                 int max_query_len, hipStream_t stream);
+
+// Windowed prefill for the shapes the pair kernel does not take (window_prefill.hip).
+bool window_prefill_supported(int q_dtype, int kv_dtype, int head_dim);
+hipError_t launch_window_prefill(const PagedParams& p, int q_dtype, int kv_dtype, int head_dim,
+                                 int max_query_len, hipStream_t stream);
 
 // Whether launch_paged_prefill has a kernel for this shape; if not, prefill rows are
 // served by the decode kernel in by-row mode.

@@ -56,6 +56,7 @@
 
 #include "common.hpp"
 #include "paged_attention.hpp"
+#include "window_list.hpp"
 
 namespace mvllm {
 
@@ -162,28 +163,6 @@ struct Cursor {
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// The key list of an item whose first query stands at position p0 (paged_attention.hpp): entry v
-// at position v for v < front, v + gap from there on, front a multiple of `align`. [hole, seen) are
-// the entries that no query of the item sees: none with align 1; with align a run of `align`
-// keys always holds a key that is seen, so the page of such a run is the sequence's own still.
-struct WindowList {
-  int front, gap, hole, seen;
-};
-template <int align>
-__device__ __forceinline__ WindowList window_list(const PagedParams& p, int p0) {
-  WindowList w;
-  const int lo = max(p0 - p.window + 1, 0);  // the first key of the first query's window
-  w.front = min(p.sinks, lo);
-  w.front = (w.front + align - 1) / align * align;
-  w.gap = max(lo / align * align - w.front, 0);
-  w.seen = lo - w.gap;
-  w.hole = min(p.sinks, w.seen);
-  return w;
-}
-__device__ __forceinline__ int list_position(const WindowList& w, int v) {
-  return v < w.front ? v : v + w.gap;
-}
 
 // Share index of workgroup `bid` of `n`: workgroups are dispatched to the XCDs round
 // robin, so this gives the workgroups of one XCD consecutive shares (the items one L2
@@ -557,9 +536,7 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
 
 }  // namespace
 
-// kWindow (on the grid only: windowed items are of about one length): an item's keys are the
-// entries of its windowed list, which with no alignment to keep holds no entry that nobody sees.
-template <typename TQ, typename TKV, int D, int HCW, int HS, bool kWindow>
+template <typename TQ, typename TKV, int D, int HCW, int HS>
 __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedParams p) {
   constexpr int kThreads = 256 * HS;
   constexpr int HW = HCW * HS;                  // query heads per work item
@@ -579,7 +556,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
 
   __shared__ __align__(16) uint16_t k_lds[2][kTileKeys * kKStride];
   __shared__ __align__(16) uint16_t v_lds[2][D * kVStride];
-  __shared__ int s_prefix[kWindow ? 1 : kMaxStreamSeqs + 1];
+  __shared__ int s_prefix[kMaxStreamSeqs + 1];
 
   const int tid = threadIdx.x;
   const int wave = uniform(tid / kWave);
@@ -593,23 +570,13 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
   const int group = p.hq / p.hk;
   const int chunks = group / HW;
   const int cols = p.hk * chunks;
-  const bool stream = !kWindow && p.pf_wgs > 0;
+  const bool stream = p.pf_wgs > 0;
   int share = xcd_share(blockIdx.x, gridDim.x);
 
   // ---- this workgroup's units [u0, u1) and the cursor at u0.
   Cursor cur;
   int u0, u1;
-  if (!prefill_work<kThreads, kWindow>(p, cols, share, s_prefix, cur, u0, u1)) return;
-  // Positions below are entries of the item's key list (itself, but for kWindow).
-  WindowList list{};
-  if constexpr (kWindow) {
-    list = window_list<1>(p, cur.context - cur.len + cur.q * kPrefillQueryTile);
-    cur.context -= list.gap;
-    cur.nt = u1 = prefill_item_tiles(cur.context, cur.len, cur.q);
-    if (u1 <= 0) return;
-  }
-  auto position = [&](int v) __attribute__((always_inline)) { return kWindow ? list_position(list, v) : v; };
-  auto held = [&](int id) __attribute__((always_inline)) { return kWindow ? held_page(p, id) : id; };
+  if (!prefill_work<kThreads>(p, cols, share, s_prefix, cur, u0, u1)) return;
   auto advance = [&](Cursor& k) __attribute__((always_inline)) {
     ++k.u;
     if (++k.t < k.nt) return;
@@ -651,21 +618,21 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     const int last = k.context - 1;
     const int kvh = k.c / chunks;  // fp8 scales only
 #pragma unroll
-    for (int u = 0; u < kKUnits; ++u) kpg[S][u] = table[position(min(key0 + k_key(u), last)) >> p.block_shift];
+    for (int u = 0; u < kKUnits; ++u) kpg[S][u] = table[min(key0 + k_key(u), last) >> p.block_shift];
 #pragma unroll
     for (int u = 0; u < kVUnits; ++u) {
 #pragma unroll
       for (int j = 0; j < kVKeys; ++j) {
-        vpg[S][u][j] = table[position(min(key0 + kVKeys * v_grp(u) + j, last)) >> p.block_shift];
+        vpg[S][u][j] = table[min(key0 + kVKeys * v_grp(u) + j, last) >> p.block_shift];
       }
     }
     if constexpr (kFp8) {
 #pragma unroll
-      for (int u = 0; u < kKUnits; ++u) ksc[S][u] = p.k_scales[static_cast<int64_t>(held(kpg[S][u])) * p.hk + kvh];
+      for (int u = 0; u < kKUnits; ++u) ksc[S][u] = p.k_scales[static_cast<int64_t>(kpg[S][u]) * p.hk + kvh];
 #pragma unroll
       for (int u = 0; u < kVUnits; ++u) {
 #pragma unroll
-        for (int j = 0; j < kVKeys; ++j) vsc[S][u][j] = p.v_scales[static_cast<int64_t>(held(vpg[S][u][j])) * p.hk + kvh];
+        for (int j = 0; j < kVKeys; ++j) vsc[S][u][j] = p.v_scales[static_cast<int64_t>(vpg[S][u][j]) * p.hk + kvh];
       }
     }
   };
@@ -686,16 +653,16 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     const uint32_t head_off = static_cast<uint32_t>((k.c / chunks) * p.kv_head_bytes);
 #pragma unroll
     for (int u = 0; u < kKUnits; ++u) {
-      const int key = position(min(key0 + k_key(u), last));
-      const uint64_t off = pool_offset(held(kpg[S][u]), key, head_off + k_dim(u) * kElemBytes);
+      const int key = min(key0 + k_key(u), last);
+      const uint64_t off = pool_offset(kpg[S][u], key, head_off + k_dim(u) * kElemBytes);
       kreg[S][u] = Stage<TQ, TKV>::load(kpool + off, kFp8 ? ksc[S][u] : 1.0f);
     }
 #pragma unroll
     for (int u = 0; u < kVUnits; ++u) {
 #pragma unroll
       for (int j = 0; j < kVKeys; ++j) {
-        const int key = position(min(key0 + kVKeys * v_grp(u) + j, last));
-        const uint64_t off = pool_offset(held(vpg[S][u][j]), key, head_off + v_dim(u) * kElemBytes);
+        const int key = min(key0 + kVKeys * v_grp(u) + j, last);
+        const uint64_t off = pool_offset(vpg[S][u][j], key, head_off + v_dim(u) * kElemBytes);
         vreg[S][u][j] = Stage<TQ, TKV>::load(vpool + off, kFp8 ? vsc[S][u][j] : 1.0f);
       }
     }
@@ -789,24 +756,7 @@ __global__ __launch_bounds__(256 * HS) void paged_prefill_kernel(const PagedPara
     }
 
     // Causal mask, on tiles crossing the diagonal only: score (kb, r) of this lane is
-    // key key0 + 4*hsel + (32kb + 8(r/4) + r%4); visible while below my_visible. And the
-    // window's, on tiles that hold keys between the sinks and a query's own first one.
-    if constexpr (kWindow) {
-      if (key0 < w_kv_end - p.window && key0 + kTileKeys > p.sinks) {
-        const int lo = my_visible - p.window - key0 - 4 * hsel, front = p.sinks - key0 - 4 * hsel;
-#pragma unroll
-        for (int h = 0; h < HCW; ++h) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int e = kb * 32 + 8 * (r >> 2) + (r & 3);
-              if (e >= front && e < lo) s[h][kb][r] = -INFINITY;
-            }
-          }
-        }
-      }
-    }
+    // key key0 + 4*hsel + (32kb + 8(r/4) + r%4); visible while below my_visible.
     if (key0 + kTileKeys > w_kv_full) {
       asm volatile("" ::: "memory");  // keep this a branch: most tiles need no mask
       const int lim = my_valid ? my_visible - key0 - 4 * hsel : INT_MIN;
@@ -1422,11 +1372,16 @@ __global__ __launch_bounds__(256) void paged_prefill_lds_kernel(const PagedParam
 // no query of the item sees are staged as a seen row of their page, so nothing behind the window
 // is used, whatever it holds; a query's own window is a second comparison per score, on the one
 // or two tiles that hold a window's edge.
-template <typename TQ, typename TKV, int kWaves, bool kSplit, bool kWindow>
+//
+// kOne (windowed, on the grid): the same for groups with an odd head: an item's waves are 32
+// positions each of one query head, twice the positions of a pair's item.
+template <typename TQ, typename TKV, int kWaves, bool kSplit, bool kWindow, bool kOne = false>
 __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(const PagedParams p) {
   constexpr bool kFp8 = std::is_same_v<TKV, fp8_t>;
   constexpr int D = 128;
-  constexpr int QT = kWaves * 16;            // query positions: kWaves / 2 waves of 32 per head
+  static_assert(!kOne || (kWindow && !kSplit), "single heads: windowed items on the grid");
+  constexpr int kHeads = kOne ? 1 : 2;
+  constexpr int QT = kWaves * 32 / kHeads;   // query positions: kWaves / kHeads waves of 32 per head
   constexpr int KW = kTileKeys / kWaves;     // keys of a tile staged by one wave
   constexpr int kRawRow = kFp8 ? D : D * 2;  // bytes of one pool row
   constexpr int kRowLanes = kRawRow / 16;
@@ -1456,11 +1411,11 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
   const int lane = tid % kWave;
   const int l32 = lane & 31;
   const int hsel = lane >> 5;
-  const int hs = wave / (kWaves / 2);  // head of the pair
-  const int wq = wave % (kWaves / 2);  // 32-position query block
+  const int hs = wave / (kWaves / kHeads);  // head of the pair
+  const int wq = wave % (kWaves / kHeads);  // 32-position query block
 
   const int group = p.hq / p.hk;
-  const int chunks = group / 2;
+  const int chunks = group / kHeads;
   // ---- the work item: (sequence, column, query tile) and its key tiles [tb, te). Item
   // grid: sequence blockIdx.y, column blockIdx.x, query tiles dispatched longest first.
   // Split: the piece at position blockIdx.x / columns, column blockIdx.x % columns. Either
@@ -1532,7 +1487,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
   const int my_lo = kWindow ? my_visible - p.window : 0;             // first entry of its window
   const int w_lo_last = kWindow ? w_kv_end - p.window : 0;           // of its last query's
   const int row_base = sload(p.cu_seqlens_q + s);
-  const int head0 = kvh * group + (c % chunks) * 2 + hs;
+  const int head0 = kvh * group + (c % chunks) * kHeads + hs;
 
   // ---- staging map: copy j of a wave's keys: lane -> key kKeysPerCopy j + lane /
   // kRowLanes, 16-byte chunk lane % kRowLanes. 16-bit rows are swizzled through the source
@@ -2166,17 +2121,17 @@ __global__ __launch_bounds__(kMergeThreads) void paged_prefill_merge_kernel(cons
 
 namespace {
 
-template <typename TQ, typename TKV, int D, int HCW, int HS, bool kWindow>
+template <typename TQ, typename TKV, int D, int HCW, int HS>
 void launch_prefill_cfg(const PagedParams& p, int max_query_len, hipStream_t stream) {
   constexpr int HW = HCW * HS;
-  if (!kWindow && p.pf_wgs > 0) {
-    paged_prefill_kernel<TQ, TKV, D, HCW, HS, false><<<p.pf_wgs, 256 * HS, 0, stream>>>(p);
+  if (p.pf_wgs > 0) {
+    paged_prefill_kernel<TQ, TKV, D, HCW, HS><<<p.pf_wgs, 256 * HS, 0, stream>>>(p);
     paged_prefill_merge_kernel<TQ, D, HW><<<kMergeSub * p.pf_wgs, kMergeThreads, 0, stream>>>(p);
   } else {
     const int cols = p.hk * (p.hq / p.hk / HW);
     const int qtiles = (max_query_len + kPrefillQueryTile - 1) / kPrefillQueryTile;
     const dim3 grid(cols, p.num_seqs, qtiles);
-    paged_prefill_kernel<TQ, TKV, D, HCW, HS, kWindow><<<grid, 256 * HS, 0, stream>>>(p);
+    paged_prefill_kernel<TQ, TKV, D, HCW, HS><<<grid, 256 * HS, 0, stream>>>(p);
   }
 }
 
@@ -2235,24 +2190,24 @@ hipError_t launch_prefill_d(const PagedParams& p, int max_query_len, hipStream_t
         else launch_prefill_pair<TQ, TKV, false>(p, max_query_len, stream);
         return hipGetLastError();
       }
+      if (p.window > 0) {
+        const dim3 grid(p.hq, p.num_seqs, (max_query_len + 127) / 128);
+        paged_prefill_pair_kernel<TQ, TKV, 4, false, true, true><<<grid, 256, 0, stream>>>(p);
+        return hipGetLastError();
+      }
       if constexpr (std::is_same_v<TQ, TKV>) {
-        if (p.window == 0) {
-          launch_prefill_lds<TQ>(p, max_query_len, stream);
-          return hipGetLastError();
-        }
+        launch_prefill_lds<TQ>(p, max_query_len, stream);
+        return hipGetLastError();
       }
     }
   }
   // Both heads of an even GQA group in one wave (HCW = 2) would share K/V fragments,
   // but needs ~450 registers: one wave per SIMD and no softmax/MFMA overlap. Measured
   // at config 3 it ran 25-40% slower than a wave per head, two waves per SIMD.
-  const bool one = prefill_item_heads(p.hq / p.hk) == 1;
-  if (p.window > 0) {
-    if (one) launch_prefill_cfg<TQ, TKV, D, 1, 1, true>(p, max_query_len, stream);
-    else launch_prefill_cfg<TQ, TKV, D, 1, 2, true>(p, max_query_len, stream);
+  if (prefill_item_heads(p.hq / p.hk) == 1) {
+    launch_prefill_cfg<TQ, TKV, D, 1, 1>(p, max_query_len, stream);
   } else {
-    if (one) launch_prefill_cfg<TQ, TKV, D, 1, 1, false>(p, max_query_len, stream);
-    else launch_prefill_cfg<TQ, TKV, D, 1, 2, false>(p, max_query_len, stream);
+    launch_prefill_cfg<TQ, TKV, D, 1, 2>(p, max_query_len, stream);
   }
   return hipGetLastError();
 }
@@ -2282,6 +2237,10 @@ bool paged_prefill_supported(int q_dtype, int kv_dtype, int head_dim, int hq, in
 
 hipError_t launch_paged_prefill(const PagedParams& p, int q_dtype, int kv_dtype, int head_dim,
                                 int max_query_len, hipStream_t stream) {
+  // (windowed: what the pair kernel does not take, by the same conditions as below)
+  if (p.window > 0 && !(head_dim == 128 && p.block_shift >= 4 && p.scale > 0.0f && !p.pf_register_staging)) {
+    return launch_window_prefill(p, q_dtype, kv_dtype, head_dim, max_query_len, stream);
+  }
   if (q_dtype == kBF16) {
     if (kv_dtype == kFP8E4M3) return launch_prefill_t<bf16_t, fp8_t>(p, head_dim, max_query_len, stream);
     return launch_prefill_t<bf16_t, bf16_t>(p, head_dim, max_query_len, stream);
