@@ -276,11 +276,16 @@ struct PairMode {
   int tile;
   bool cut;
 };
-PairMode pair_mode(const PairWork& w, int32_t num_seqs, int32_t hq, int32_t max_q, int32_t kv_dtype, int cus) {
+// Windowed items are of about one length, so that past two and a half a CU more smaller ones fill the
+// rounds better: four fresh prompts of 4096 over fp8, window 1024, 172 us with items of 64 and 184 with
+// 128; 512 items of 8 x 512 56 and 53.
+PairMode pair_mode(const PairWork& w, int32_t num_seqs, int32_t hq, int32_t max_q, int32_t kv_dtype, int cus,
+                   bool windowed) {
   const bool fp8 = kv_dtype == mvllm::kFP8E4M3;
   // A grid of very many positions is halved (1500 decodes and 2048 tokens, 384K: 738 -> 700 us).
   const bool vast = static_cast<int64_t>(num_seqs) * ((max_q + 63) / 64) * (hq / 2) >= 128 * 1024;
-  const bool wide = fp8 && ((2 * w.wgs >= 3 * cus && max_q <= 32 * w.n) || 2 * w.wgs >= 5 * cus);
+  const bool wide = windowed ? fp8 && 2 * w.wgs >= 3 * cus && 2 * w.wgs < 5 * cus
+                             : fp8 && ((2 * w.wgs >= 3 * cus && max_q <= 32 * w.n) || 2 * w.wgs >= 5 * cus);
   const PairMode whole{max_q > 64 && (vast || wide) ? 128 : 64, false};
   // Past 64 sequences the schedule is a launch of its own, and the list and the merge have a
   // position per sequence and column: about 6 us and 1.5 ns each.
@@ -354,7 +359,7 @@ void plan_prefill(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, 
     if (!pair) return;  // (the other kernels run windowed items whole, on the item grid)
   }
   const PairWork work = pair_work(num_tokens, num_seqs, hq, max_q, static_cast<int32_t>(span), windowed);
-  const PairMode m = pair_mode(work, num_seqs, hq, max_q, kv_dtype, cus);
+  const PairMode m = pair_mode(work, num_seqs, hq, max_q, kv_dtype, cus, windowed);
   const int64_t qtiles = (static_cast<int64_t>(num_tokens) + mvllm::kPrefillQueryTile - 1) /
                          mvllm::kPrefillQueryTile;
   const int64_t items = qtiles * (hq / mvllm::prefill_item_heads(hq / hk));

@@ -206,7 +206,7 @@ __device__ __forceinline__ float finite_max(float m, const float (&x)[E]) {
 // in LDS (the order of a maximum does not matter). So a run's rows, angles and old scale are
 // requested one round trip after the launch, and 16 single tokens take as long as a page of 16.
 // One run after another, each finding its slots, length, positions and angles in turn, and q's
-// workgroups last: 8704 tokens in eight chunks 37.7 us, now 31.4 (4.3 TB/s); 128 tokens 10.3, now 6.5;
+// workgroups last: 9637 tokens in eight chunks 37.7 us, now 35.4 (4.2 TB/s); 128 tokens 10.3, now 6.5;
 // 2048 single tokens 44.9, now 11.9; 64 level at 4.4.
 template <typename T, typename TPos, int D, int G>
 __global__ __launch_bounds__(256) void rope_write_fp8_kernel(const RopeWriteParams p, int every,
