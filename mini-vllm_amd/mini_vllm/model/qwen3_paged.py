@@ -56,6 +56,10 @@ class ModelConfig:
     rms_norm_eps: float = 1e-6
     rope_theta: float = 1_000_000.0
     dtype: torch.dtype = torch.bfloat16
+    # Every layer's attention over the newest `sliding_window` keys and the sequence's first
+    # `attention_sinks` (None: over every key; no counterpart in the reference).
+    sliding_window: int | None = None
+    attention_sinks: int = 0
 
     @property
     def q_size(self) -> int:
@@ -190,7 +194,7 @@ class Qwen3Paged:
         """The attention output (``T x H_q D``) of normed input x, before ``wo``."""
         c = self.config
         q, k, v = self._projections(w, p, x, fused)
-        if fused and batch.max_query_len == 1:
+        if fused and batch.max_query_len == 1 and c.sliding_window is None:
             # A decode step: QK-norm, RoPE and the KV write inside the attention launch.
             kv = self.manager.kv
             out = ops.paged_decode_qk_norm_rope(
@@ -241,11 +245,17 @@ class Qwen3Paged:
         c = self.config
         kv = self.manager.kv
         k_scale, v_scale = kv.layer_scales(layer)
-        out = ops.paged_attention(
-            q, kv.layer_keys(layer), kv.layer_values(layer), batch.block_tables,
-            batch.cu_seqlens_q, batch.context_lens, batch.seq_lens, batch.max_query_len,
-            batch.max_context_len, 1.0 / math.sqrt(c.head_dim), use_cuda=self.use_cuda,
-            k_scale=k_scale, v_scale=v_scale)
+        args = (q, kv.layer_keys(layer), kv.layer_values(layer), batch.block_tables,
+                batch.cu_seqlens_q, batch.context_lens, batch.seq_lens, batch.max_query_len,
+                batch.max_context_len)
+        scale = 1.0 / math.sqrt(c.head_dim)
+        if c.sliding_window is None:
+            out = ops.paged_attention(*args, scale, use_cuda=self.use_cuda, k_scale=k_scale,
+                                      v_scale=v_scale)
+        else:
+            out = ops.paged_window_attention(*args, c.sliding_window, c.attention_sinks, scale,
+                                             use_cuda=self.use_cuda, k_scale=k_scale,
+                                             v_scale=v_scale)
         return out.view(q.shape[0], c.q_size)
 
     def _residual_norm(self, x: torch.Tensor, pw, dense_w: torch.Tensor, h: torch.Tensor,

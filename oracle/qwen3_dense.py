@@ -7,6 +7,9 @@ kernels, so a paged engine that agrees with it token for token got its batching,
 slots, positions and masks right. Returns the tokens and each step's logits so a test
 can tell a genuine near-tie from a bug.
 
+:func:`generate_greedy` also takes a config with a sliding window and sinks (the cached forms
+take none).
+
 ``DenseQwen3(..., kv_fp8=True)`` is the same model with its K/V cache held the way an
 fp8-e4m3 paged pool holds it (the reference has no fp8 cache): every K/V row written
 through ``oracle.kv_write.kv_write_fp8`` (per-(page, kv head) power-of-two scales,
@@ -47,6 +50,9 @@ def _forward_last(config, w, ids, dtype):
     pos = torch.arange(t)
     g = c.num_attention_heads // c.num_key_value_heads
     mask = torch.full((t, t), float("-inf"), dtype=dtype).triu(1)
+    if c.sliding_window is not None:  # the newest keys and the first ones
+        behind = pos[:, None] - pos[None] >= c.sliding_window
+        mask[behind & (pos[None] >= c.attention_sinks)] = float("-inf")
     for layer in range(c.num_hidden_layers):
         lw = {k.split(".", 2)[2]: v.to(dtype) for k, v in w.items() if k.startswith(f"layers.{layer}.")}
         x = _rms(h, lw["attn_norm"], c.rms_norm_eps)
