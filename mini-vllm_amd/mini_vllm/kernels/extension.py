@@ -573,7 +573,8 @@ class HipExtension:
         return self._host.paged_decode_qk_norm_rope(self._entries, self._workspaces, *args)
 
     def try_paged_window_attention(self, *args):
-        if self._host is None or self._recording is not None:
+        if (self._host is None or self._recording is not None
+                or torch.cuda.is_current_stream_capturing()):
             return None
         return self._host.paged_window_attention(self._rolling, self._workspaces, *args)
 
@@ -1783,7 +1784,13 @@ class HipExtension:
                 *sizes, int(max_query_len), int(max_context_len), window, sinks, *codes, opts_ref,
                 ctypes.byref(plan)))
             workspace = None
-            if plan.workspace_bytes:
+            if plan.workspace_bytes and torch.cuda.is_current_stream_capturing():
+                # of the graph's own pool: what is eager on the stream, and other graphs, have
+                # other memory
+                workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=q.device)
+                if self._recording is not None:
+                    self._recording.append(workspace)
+            elif plan.workspace_bytes:
                 workspace = self.workspace(q.device, plan.workspace_bytes)
             self._check(self.lib.mvllm_paged_window_attention(
                 out.data_ptr(), q.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),

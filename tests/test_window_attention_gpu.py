@@ -208,6 +208,36 @@ def test_captured_and_replayed_on_another_stream(device, pairs):
         torch.cuda.synchronize()
 
 
+def test_two_graphs_and_eager_calls_share_no_workspace(device):
+    """Two graphs captured on one stream that has no workspace yet, replayed side by side on two
+    streams, then after a larger eager call has grown that stream's workspace."""
+    cases = [on(rolling_batch(pairs, 4000, 4, dtype=torch.bfloat16), device)
+             for pairs in ([(5000, 1)], [(4500, 1), (900, 200)])]
+    large = on(rolling_batch([(5000, 1)] * 3 + [(4000, 500)], 4000, 4, dtype=torch.bfloat16), device)
+    want = [call(b, device).clone() for b in cases]
+    large_want = call(large, device).clone()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    graphs, outs = [], []
+    for b in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            outs.append(call(b, device))
+        graphs.append(graph)
+    for round_ in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams[1:]):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        if round_ > 0:
+            with torch.cuda.stream(streams[0]):
+                got = call(large, device)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]), round_
+        assert round_ == 0 or torch.equal(got, large_want)
+
+
 @pytest.mark.parametrize("dtype,kv_dtype", [TYPES[0], TYPES[2], TYPES[4]])
 @pytest.mark.parametrize("d", [64, 128])
 def test_a_freed_page_that_is_seen_reads_within_the_pool(device, d, dtype, kv_dtype):
