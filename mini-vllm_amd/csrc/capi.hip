@@ -531,6 +531,8 @@ int launch_planned(const Plan& plan, mvllm::PagedParams& p, void* workspace, int
   p.split_tokens = plan.pub.split_tokens > 0 ? plan.pub.split_tokens : mvllm::kMaxSplitTokens;
   p.max_splits = plan.max_splits;
   p.by_row = plan.pub.decode_mode == MVLLM_DECODE_BY_ROW ? 1 : 0;
+  // (every sequence a chunk, by the count of q's rows: which may hold rows of no sequence)
+  p.pf_min_len = plan.pub.decode_mode == MVLLM_DECODE_NONE ? 1 : 2;
   p.pf_register_staging = plan.register_staging;
   p.pf_share_tiles = plan.prefill_share_tiles;
   if (plan.pub.workspace_bytes > 0) {

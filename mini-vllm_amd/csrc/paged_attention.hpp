@@ -222,6 +222,8 @@ struct PagedParams {
   int window;         // > 0: windowed attention (the kernels' kWindow forms): a query at
   int sinks;          // position p sees the keys j <= p with j > p - window or j < sinks
                       // (sinks + window < 2^31)
+  int pf_min_len;     // windowed prefill: fewest query tokens of a sequence that are its work: 2, or
+                      // 1 where no decode kernel is launched
   int direct;         // windowed decode: 1 selects the direct schedule
   uint32_t last_block;  // windowed: the pool's last page, which an id outside the pool is read as
 };

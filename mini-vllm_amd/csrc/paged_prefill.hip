@@ -303,9 +303,16 @@ __device__ __forceinline__ int pair_item_tiles(const PagedParams& p, int context
   return (end + kTileKeys - 1) / kTileKeys;
 }
 
+// Whether a sequence's rows are the prefill's (a decode row is the decode kernel's, unless a
+// windowed launch has none).
+template <bool kWindow>
+__device__ __forceinline__ bool is_chunk(const PagedParams& p, int len) {
+  return kWindow ? len >= p.pf_min_len : len > 1;
+}
 // Query tiles of a sequence (a decode row has none here).
-__device__ __forceinline__ int pair_query_tiles(int len, int qt) {
-  return len > 1 ? (len + qt - 1) / qt : 0;
+template <bool kWindow>
+__device__ __forceinline__ int pair_query_tiles(const PagedParams& p, int len, int qt) {
+  return is_chunk<kWindow>(p, len) ? (len + qt - 1) / qt : 0;
 }
 
 // The schedule's piece length in tiles: pct% of the mean tiles per CU of all items, at least
@@ -323,8 +330,10 @@ __device__ __forceinline__ bool pair_stays_whole(const PagedParams& p, int cols,
   return p.pf_weigh != 0 && static_cast<int64_t>(longest) * c.whole * p.pf_cus <=
                                 static_cast<int64_t>(total) * cols * c.cut + c.weigh * static_cast<int64_t>(p.pf_cus);
 }
+template <bool kWindow>
 __device__ __forceinline__ int pair_pieces(const PagedParams& p, int nt, int length) {
-  return min(p.pf_pieces, (nt + length - 1) / length);
+  const int pieces = min(p.pf_pieces, (nt + length - 1) / length);
+  return kWindow ? max(pieces, 1) : pieces;  // (an item without a key has rows of zeros to write)
 }
 
 // Whether to stop at this length: all pieces run at once, or longer ones change nothing or
@@ -338,10 +347,10 @@ __device__ __forceinline__ bool pair_fits(const PagedParams& p, int cols, int ra
 // Pieces (low half) and cut items' slots (high half; both below 2^15) of a sequence.
 template <int QT, bool kWindow>
 __device__ __forceinline__ int pair_count(const PagedParams& p, int ctx, int len, int length) {
-  const int qts = pair_query_tiles(len, QT);
+  const int qts = pair_query_tiles<kWindow>(p, len, QT);
   int both = 0;
   for (int q = 0; q < qts; ++q) {
-    const int pcs = pair_pieces(p, pair_item_tiles<kWindow>(p, ctx, len, q, QT), length);
+    const int pcs = pair_pieces<kWindow>(p, pair_item_tiles<kWindow>(p, ctx, len, q, QT), length);
     both += pcs | (pcs > 1 ? pcs << 16 : 0);
   }
   return both;
@@ -353,7 +362,7 @@ __device__ __forceinline__ void pair_locate(const PagedParams& p, int ctx, int l
                                             PairPiece& out) {
   for (out.q = 0;; ++out.q) {
     const int nt = pair_item_tiles<kWindow>(p, ctx, len, out.q, QT);
-    out.pieces = pair_pieces(p, nt, length);
+    out.pieces = pair_pieces<kWindow>(p, nt, length);
     if (r < out.pieces) {
       out.piece = r;
       out.tb = r * nt / out.pieces;
@@ -378,7 +387,7 @@ __device__ __forceinline__ bool pair_piece(const PagedParams& p, int cols, int r
   auto wave_total = [&](int v) __attribute__((always_inline)) -> int {
     return __builtin_amdgcn_readlane(wave_inclusive_scan(v), kWave - 1);
   };
-  const int qts = pair_query_tiles(len, QT);
+  const int qts = pair_query_tiles<kWindow>(p, len, QT);
   if (p.pf_pieces == 1) {
     // Whole items, longest first: by sequence, or every sequence's last query tile, then every
     // one's before it, and so on.
@@ -467,10 +476,10 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int s = base + i * kWave + lane;
-      const uint64_t have = __builtin_amdgcn_ballot_w64(s < n && len[i] > 1);
+      const uint64_t have = __builtin_amdgcn_ballot_w64(s < n && is_chunk<kWindow>(p, len[i]));
       const int nth = static_cast<int>(__builtin_amdgcn_mbcnt_hi(
           static_cast<uint32_t>(have >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(have), 0)));
-      if (s < n && len[i] > 1) {
+      if (s < n && is_chunk<kWindow>(p, len[i])) {
         s_seq[chunks + nth] = s;
         s_len[chunks + nth] = len[i];
         s_ctx[chunks + nth] = ctx[i];
@@ -487,7 +496,7 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
   int total = 0, items = 0, longest = 0;
   for (int base = 0; base < chunks; base += kWave) {
     take(base);
-    const int qts = pair_query_tiles(len, QT);
+    const int qts = pair_query_tiles<kWindow>(p, len, QT);
     int tiles = 0;
     for (int q = 0; q < qts; ++q) tiles += pair_item_tiles<kWindow>(p, ctx, len, q, QT);
     const int own = qts > 0 ? pair_item_tiles<kWindow>(p, ctx, len, qts - 1, QT) : 0;
@@ -513,12 +522,12 @@ __global__ __launch_bounds__(kWave) void paged_prefill_schedule_kernel(const Pag
     const int incl = wave_inclusive_scan(both);
     const int all = __builtin_amdgcn_readlane(incl, kWave - 1);
     int rank = ranks + ((incl - both) & 0xffff), slot0 = slots + ((incl - both) >> 16);
-    const int qts = pair_query_tiles(len, QT);
+    const int qts = pair_query_tiles<kWindow>(p, len, QT);
     PairPiece w{};
     w.s = base + lane < chunks ? s_seq[base + lane] : 0;
     for (w.q = 0; w.q < qts; ++w.q) {
       const int nt = pair_item_tiles<kWindow>(p, ctx, len, w.q, QT);
-      w.pieces = pair_pieces(p, nt, length);
+      w.pieces = pair_pieces<kWindow>(p, nt, length);
       w.slot0 = slot0;
       if (w.pieces > 1) slot0 += w.pieces;
       const bool fits = w.pieces == 1 || slot0 <= p.pf_slots;  // (the host's bounds see to both)
@@ -1451,11 +1460,21 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
   const int len = sload(p.seq_lens + s);
   const int held = sload(p.context_lens + s);
   if constexpr (!kSplit) {
-    if (len <= 1) return;  // a decode row: the decode kernel has it
+    if (!is_chunk<kWindow>(p, len)) return;
     if (qt * QT >= len) return;
     tb = 0;
     te = pair_item_tiles<kWindow>(p, held, len, qt, QT);
-    if (kWindow && te <= 0) return;
+  }
+  if constexpr (kWindow) {
+    if (te <= tb) {  // no key at all: zeros
+      const int first = sload(p.cu_seqlens_q + s) + qt * QT, rows = min(QT, len - qt * QT);
+      const int head = c / chunks * group + c % chunks * kHeads;
+      for (int i = tid; i < rows * kHeads * D / 2; i += kWaves * kWave) {
+        const int64_t row = (static_cast<int64_t>(first) + i / (kHeads * D / 2)) * p.hq + head;
+        static_cast<uint32_t*>(p.out)[row * (D / 2) + i % (kHeads * D / 2)] = 0;
+      }
+      return;
+    }
   }
   // Positions below are entries of the item's key list (itself, but for kWindow).
   WindowList list{};

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void window_prefill_kernel(const
 
   const int seq = blockIdx.y, kvh = blockIdx.x;
   const int len = sload(p.seq_lens + seq);
-  if (len <= 1) return;  // a decode row: the decode kernel has it
+  if (len < p.pf_min_len) return;  // a decode row: the decode kernel has it
   const int held = sload(p.context_lens + seq);
   const int group = p.hq / p.hk;
   const int rows = len * group;
@@ -112,13 +112,21 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void window_prefill_kernel(const
   const int item = (rows + kRows - 1) / kRows - 1 - static_cast<int>(blockIdx.z);
   if (item < 0) return;
   const int row0 = item * kRows, row_end = min(row0 + kRows, rows);
+  const int q_row0 = sload(p.cu_seqlens_q + seq);
   const int offset = held - len;
   const WindowList list = window_list<1>(p, offset + row0 / group);
   const int keys = offset + (row_end - 1) / group + 1 - list.gap;  // entries the item walks
   const int tiles = (keys + kTile - 1) / kTile;
-  if (tiles <= 0) return;
 
   const int tid = threadIdx.x, lane = tid % kWave;
+  if (tiles <= 0) {  // no key at all: zeros
+    for (int i = tid; i < (row_end - row0) * (D / 2); i += kThreads) {
+      const int row = row0 + i / (D / 2), at = row / group;
+      const int64_t head = static_cast<int64_t>(q_row0 + at) * p.hq + kvh * group + (row - at * group);
+      static_cast<uint32_t*>(p.out)[head * (D / 2) + i % (D / 2)] = 0;
+    }
+    return;
+  }
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int n16 = lane & 15, g = lane >> 4;
 
@@ -129,7 +137,6 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void window_prefill_kernel(const
   const int w_full = offset + w_row0 / group + 1 - list.gap;          // entries all its rows see
   const int w_end = w_active ? offset + w_last / group + 1 - list.gap : 0;
   int visible[kBlocks];
-  const int q_row0 = sload(p.cu_seqlens_q + seq);
   u32x4 qop[kBlocks][kSteps];
   const float raw_c = p.scale * kLog2e;
   const float score_c = fmaxf(fabsf(raw_c), 1e-30f);  // (a negative scale's sign is moved into Q)

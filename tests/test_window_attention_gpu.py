@@ -162,6 +162,25 @@ def test_rows_behind_the_last_sequence_stay(device, extension, pairs, dtype):
     assert bool((out[-5:] == 7.0).all())
 
 
+@pytest.mark.parametrize("hq,hk,d,page", [(4, 2, 128, 16), (3, 1, 128, 16), (4, 2, 64, 16), (4, 2, 128, 8)])
+@pytest.mark.parametrize("pairs,spare", [([(90, 2), (50, 1)], 1), ([(90, 2), (0, 1)], 1),
+                                         ([(200, 64), (30, 1), (0, 1)], 126),
+                                         ([(300, 3)] + [(i, 1) for i in range(70)], 140)])
+def test_padded_queries_that_look_like_chunks_only(device, extension, pairs, spare, hq, hk, d, page):
+    """q holding rows of no sequence, as many as make its count that of chunks alone."""
+    b = rolling_batch(pairs, 30, 4, dtype=torch.bfloat16, hq=hq, hk=hk, d=d, page=page, spare_rows=spare)
+    assert b["q"].shape[0] == len(pairs) * b["max_query_len"]
+    args = on(b, device)
+    for options in (None, {"prefill_schedule": 1, "prefill_share_tiles": 1}):
+        out = torch.full_like(args["q"], 7.0)
+        extension.paged_window_attention(
+            args["q"], args["key_pool"], args["value_pool"], args["block_tables"],
+            args["cu_seqlens_q"], args["context_lens"], args["seq_lens"], b["max_query_len"],
+            b["max_context_len"], 30, 4, b["scale"], out=out, plan_options=options)
+        assert_close(out, b, str(options), chunks_only=True)
+        assert bool((out[-spare:] == 7.0).all())
+
+
 def test_misaligned_queries_and_refusals(device, extension):
     b = on(rolling_batch(MIXED, 30, 4, dtype=torch.bfloat16, hq=4, hk=2), device)
     shifted = torch.empty(b["q"].numel() + 1, dtype=torch.bfloat16, device=device)[1:].view(b["q"].shape)

@@ -66,8 +66,9 @@ def on(batch, device):
     return {k: v.to(device) if isinstance(v, torch.Tensor) else v for k, v in batch.items()}
 
 
-def expected(batch):
-    """The oracle's outputs and the most a kernel may be off, element by element.
+def expected(batch, chunks_only=False):
+    """The oracle's outputs and the most a kernel may be off, element by element (``chunks_only``:
+    single queries are computed as chunks of one token).
 
     The sums are in float32: a score of D terms is off by (D + 2) 2^-24 of their size, and so is
     the exponent by that and by its own rounding (at most 2^-22 of the score's size, log2 e and the
@@ -90,7 +91,7 @@ def expected(batch):
     if q.dtype != torch.float32:
         cu = batch["cu_seqlens_q"].tolist()
         for s, l in enumerate(batch["seq_lens"].tolist()):
-            if l > 1:
+            if l > 1 or chunks_only:
                 weight[cu[s]:cu[s + 1]] = half
         if batch["k_scale"] is not None and not torch.equal(
                 batch["k_scale"], torch.exp2(torch.round(torch.log2(batch["k_scale"])))):
@@ -105,8 +106,8 @@ def expected(batch):
     return out, tolerance + 1e-30
 
 
-def assert_close(actual, batch, msg=""):
-    out, tolerance = expected(batch)
+def assert_close(actual, batch, msg="", chunks_only=False):
+    out, tolerance = expected(batch, chunks_only)
     rows = int(batch["cu_seqlens_q"][-1])
     got = actual.double().cpu()[:rows]
     assert torch.isfinite(got).all(), f"{msg}: non-finite output"
