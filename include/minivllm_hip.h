@@ -59,9 +59,10 @@ const char* mvllm_build_id(void);
 #define MVLLM_DECODE_GRID 2   /* one workgroup per (sequence, split) */
 #define MVLLM_DECODE_BY_ROW 3 /* one workgroup per (query row, split), prefill rows too */
 #define MVLLM_DECODE_DIRECT 4 /* windowed calls: one workgroup per (sequence, kv head) */
+#define MVLLM_DECODE_BESIDE 5 /* windowed calls: the same, in the prefill kernel's launch */
 typedef struct mvllm_paged_plan {
   int32_t decode_mode;       /* MVLLM_DECODE_* */
-  int32_t decode_workgroups; /* stream, direct: workgroups launched; grid modes: split-axis
+  int32_t decode_workgroups; /* stream, direct, beside: workgroups launched; grid modes: split-axis
                                 extent */
   int32_t split_tokens;      /* grid modes: keys per split */
   int32_t prefill_mfma;      /* 1: prefill rows go to the MFMA prefill kernel */
@@ -88,7 +89,8 @@ typedef struct mvllm_paged_plan {
  * the sizes, the device's CU count and these options only. */
 typedef struct mvllm_plan_options {
   int32_t decode_schedule;     /* 0 auto; MVLLM_DECODE_STREAM, MVLLM_DECODE_GRID or, of a
-                                  windowed call, MVLLM_DECODE_DIRECT forces one */
+                                  windowed call, MVLLM_DECODE_DIRECT or (with chunks that
+                                  the GQA-pair kernel takes) MVLLM_DECODE_BESIDE forces one */
   int32_t decode_wgs_per_cu;   /* stream decode: workgroups per CU (default 1) */
   int32_t decode_waves_per_cu; /* grid decode: waves per CU the splits aim for (default 16) */
   int32_t decode_split_tokens; /* grid decode: keys per split (default from the wave target) */

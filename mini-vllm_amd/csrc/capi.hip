@@ -85,7 +85,8 @@ int read_options(const mvllm_plan_options* o, Options& out, bool windowed = fals
   out = Options{};
   if (o == nullptr) return MVLLM_OK;
   if (o->decode_schedule < 0 || (o->decode_schedule > MVLLM_DECODE_GRID &&
-                                 !(windowed && o->decode_schedule == MVLLM_DECODE_DIRECT)) ||
+                                 !(windowed && o->decode_schedule <= MVLLM_DECODE_BESIDE &&
+                                   o->decode_schedule >= MVLLM_DECODE_DIRECT)) ||
       o->prefill_schedule < 0 || o->prefill_schedule > 2 || o->prefill_staging < 0 ||
       o->prefill_staging > 1 || o->decode_wgs_per_cu < 0 || o->decode_waves_per_cu < 0 ||
       o->decode_split_tokens < 0 || o->prefill_wgs_per_cu < 0 || o->prefill_share_tiles < 0 ||
@@ -332,6 +333,13 @@ struct Window {
   int32_t sinks = 0;
 };
 
+// The keys that a windowed item of 64 queries walks, at most: the sinks, a window and the queries, with
+// the runs of 16 that they begin and end in.
+int32_t window_span(int32_t max_ctx, const Window& win) {
+  const int64_t list = static_cast<int64_t>(win.sinks) + 15 + win.window + 15 + 63;
+  return list < max_ctx ? static_cast<int32_t>(list) : max_ctx;
+}
+
 // The MFMA prefill's schedule, from host sizes: the grid where its 128-query items, ceil(
 // num_tokens / 128) query tiles per kv column, reach half the CU count, the stream schedule
 // (balanced shares of all key tiles) below; the prefill_schedule option 1 / 2 forces
@@ -351,14 +359,9 @@ void plan_prefill(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, 
   const int cus = device_cus();
   const bool pair = pair_prefill(hq, hk, d, block_size, q_dtype, kv_dtype, o);
   const bool windowed = win.window > 0;
-  int64_t span = max_ctx;
-  if (windowed) {
-    // The sinks, a window and the item's queries, with the runs of 16 that they begin and end in.
-    const int64_t list = static_cast<int64_t>(win.sinks) + 15 + win.window + 15 + 63;
-    if (list < span) span = list;
-    if (!pair) return;  // (the other kernels run windowed items whole, on the item grid)
-  }
-  const PairWork work = pair_work(num_tokens, num_seqs, hq, max_q, static_cast<int32_t>(span), windowed);
+  if (windowed && !pair) return;  // (the other kernels run windowed items whole, on the item grid)
+  const PairWork work =
+      pair_work(num_tokens, num_seqs, hq, max_q, windowed ? window_span(max_ctx, win) : max_ctx, windowed);
   const PairMode m = pair_mode(work, num_seqs, hq, max_q, kv_dtype, cus, windowed);
   const int64_t qtiles = (static_cast<int64_t>(num_tokens) + mvllm::kPrefillQueryTile - 1) /
                          mvllm::kPrefillQueryTile;
@@ -401,14 +404,70 @@ void plan_prefill(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, 
   }
 }
 
+// Workgroups of a sequence's decode row: a kv head's query heads in chunks.
+int64_t decode_units(int32_t hq, int32_t hk) {
+  return static_cast<int64_t>(hk) * (hq / hk / mvllm::decode_group_chunk(hq / hk));
+}
+
+// Query lengths are at most max_q and sum to num_tokens, so num_tokens == num_seqs * max_q (with
+// max_q > 1) means every sequence is a prefill chunk.
+bool all_chunks(int32_t num_tokens, int32_t num_seqs, int32_t max_q) {
+  return max_q > 1 && static_cast<int64_t>(num_seqs) * max_q == static_cast<int64_t>(num_tokens);
+}
+
+// Windowed decode rows as workgroups of the pair prefill's launch, where they run on what the items
+// leave idle: instead of a launch or two before it, but with the prefill's 4 waves a list, two
+// workgroups a CU. Worth it while a list, 4.5 us and 22 bytes a ns (17 over fp8), ends within the
+// launches that it takes the place of (three quarters of a cut prefill, whose pieces leave no CU idle),
+// and while lists are not most of the work.
+// Before and beside, us, rows of window 1024 but where said and a chunk of 512: bf16, 8 rows 44 and 29,
+// 31 53 and 35, 62 and a chunk of 256 74 and 69, 100 and four chunks 120 and 109, 20 and 8 of 256 52 and
+// 43, 30 (window 2048) and four 94 and 79; fp8, 48 and 36, 50 and 45, 60 and 54, 104 and 94, 61 and 43,
+// 109 and 73; one row and a chunk of 64, 32 and 27.
+// What the rule leaves out: that over bf16, 30 and 33; 16 rows of 2000 63 and 70; 31 of 4096 127 and
+// 133, over fp8 106 and 112; 4 of 4096 and a chunk of 1024 90 and 118, 92 and 107; and with eight chunks
+// 250 rows of 512 130 and 135, 108 and 148, over fp8 126 rows of 1000 114 and 145.
+constexpr int kBesideKeys = 2048;
+bool beside_prefill(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int32_t d, int32_t block_size,
+                    int32_t max_q, int32_t max_ctx, int32_t keys, int32_t q_dtype, int32_t kv_dtype,
+                    const Options& o, const Window& win) {
+  if (max_q <= 1 || num_seqs < 1 || num_seqs >= 65536 || all_chunks(num_tokens, num_seqs, max_q) ||
+      !pair_prefill(hq, hk, d, block_size, q_dtype, kv_dtype, o)) {
+    return false;
+  }
+  if (o.decode_schedule != 0) return o.decode_schedule == MVLLM_DECODE_BESIDE;
+  const int cus = device_cus();
+  const PairWork w = pair_work(num_tokens, num_seqs, hq, max_q, window_span(max_ctx, win), true);
+  // (no more rows than the tokens leave beside the fewest chunks)
+  const int64_t lists = (num_seqs - w.chunks) * decode_units(hq, hk);
+  const bool fp8 = kv_dtype == mvllm::kFP8E4M3;
+  if (lists < 1 || keys > kBesideKeys || lists > 4 * cus) return false;
+  if (fp8 && lists > 2 * cus && lists + w.wgs > 5 * cus) return false;
+  const mvllm::PairCosts c = mvllm::pair_costs(64, fp8);  // (in 10 ns)
+  const double share = static_cast<double>(w.wgs) / cus;
+  const double prefill = pair_mode(w, num_seqs, hq, max_q, kv_dtype, cus, true).cut
+                             ? 7.5 * (static_cast<double>(c.cut * w.n) * share + c.fixed)
+                             : 10.0 * static_cast<double>(c.whole * w.n) * (share > 1.0 ? share : 1.0);
+  const double list = 2.0 * static_cast<double>(keys) * d * element_bytes(kv_dtype);
+  const double rows = 10e3 + list * static_cast<double>(lists) / 6200;
+  return 4.5e3 + list / (fp8 ? 17 : 22) <= prefill + rows;
+}
+
 Plan make_plan(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int32_t d,
                int32_t block_size, int32_t max_q, int32_t max_ctx, int32_t q_dtype,
                int32_t kv_dtype, const Options& o = Options{}, const Window& win = Window{}) {
   Plan plan{};
   // A single query's keys: its context, or its windowed list.
   const int32_t keys = win.window > 0 ? mvllm::window_keys(max_ctx, win.window, win.sinks) : max_ctx;
-  plan_decode(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, keys, q_dtype, kv_dtype, o,
-              win.window > 0);
+  if (win.window > 0 && beside_prefill(num_tokens, num_seqs, hq, hk, d, block_size, max_q, max_ctx, keys,
+                                       q_dtype, kv_dtype, o, win)) {
+    plan.pub.decode_mode = MVLLM_DECODE_BESIDE;
+    plan.pub.decode_workgroups = static_cast<int32_t>(num_seqs * decode_units(hq, hk));
+    plan.pub.prefill_mfma = 1;
+  } else {
+    plan_decode(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, keys, q_dtype, kv_dtype, o,
+                win.window > 0);
+  }
   plan_prefill(plan, num_tokens, num_seqs, hq, hk, d, block_size, max_q, max_ctx, q_dtype, kv_dtype,
                o, win);
   if (plan.pub.prefill_mfma && pair_prefill(hq, hk, d, block_size, q_dtype, kv_dtype, o)) {
@@ -440,11 +499,8 @@ void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, i
   const bool mfma =
       has_prefill && (windowed ? mvllm::window_prefill_supported(q_dtype, kv_dtype, d)
                                : mvllm::paged_prefill_supported(q_dtype, kv_dtype, d, hq, hk, block_size));
-  // Query lengths are at most max_q and sum to num_tokens, so num_tokens ==
-  // num_seqs * max_q (with max_q > 1) means every sequence is a prefill chunk.
-  const bool all_prefill =
-      has_prefill && static_cast<int64_t>(num_seqs) * max_q == static_cast<int64_t>(num_tokens);
-  const int64_t units = static_cast<int64_t>(hk) * (hq / hk / mvllm::decode_group_chunk(hq / hk));
+  const bool all_prefill = all_chunks(num_tokens, num_seqs, max_q);
+  const int64_t units = decode_units(hq, hk);
   plan.pub.prefill_mfma = mfma ? 1 : 0;
 
   if (has_prefill && !mfma) {
@@ -453,7 +509,7 @@ void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, i
     plan.pub.decode_mode = MVLLM_DECODE_NONE;
   } else if (windowed && num_seqs < 65536 &&
              (o.decode_schedule == MVLLM_DECODE_DIRECT ||
-              (o.decode_schedule == 0 &&
+              ((o.decode_schedule == 0 || o.decode_schedule == MVLLM_DECODE_BESIDE) &&
                direct_decode(num_seqs * units, max_ctx, static_cast<int64_t>(d) * element_bytes(kv_dtype),
                              kv_dtype == mvllm::kFP8E4M3, device_cus())))) {
     plan.pub.decode_mode = MVLLM_DECODE_DIRECT;
@@ -526,6 +582,8 @@ int launch_planned(const Plan& plan, mvllm::PagedParams& p, void* workspace, int
                    int32_t kv_dtype, int32_t head_dim, int32_t max_query_len, hipStream_t s,
                    const char* name) {
   p.direct = plan.pub.decode_mode == MVLLM_DECODE_DIRECT ? 1 : 0;
+  // (the pair kernel takes scales above zero: without it, decode rows have their own launch)
+  if (plan.pub.decode_mode == MVLLM_DECODE_BESIDE) p.direct = p.scale > 0.0f ? 2 : 1;
   p.stream_wgs = plan.pub.decode_mode == MVLLM_DECODE_STREAM ? plan.pub.decode_workgroups : 0;
   p.stream_min_keys = mvllm::decode_min_share_keys(element_bytes(kv_dtype), head_dim);
   p.split_tokens = plan.pub.split_tokens > 0 ? plan.pub.split_tokens : mvllm::kMaxSplitTokens;
@@ -570,7 +628,7 @@ int launch_planned(const Plan& plan, mvllm::PagedParams& p, void* workspace, int
     p.pf_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.off_split);
     p.pf_rec = reinterpret_cast<int4*>(static_cast<char*>(workspace) + plan.off_rec);
   }
-  if (plan.pub.decode_mode != MVLLM_DECODE_NONE) {
+  if (plan.pub.decode_mode != MVLLM_DECODE_NONE && p.direct != 2) {
     const int rc = hip_status(mvllm::launch_paged_decode(p, q_dtype, kv_dtype, head_dim, s),
                               name);
     if (rc != MVLLM_OK) return rc;

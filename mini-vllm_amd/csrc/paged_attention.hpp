@@ -224,7 +224,8 @@ struct PagedParams {
                       // (sinks + window < 2^31)
   int pf_min_len;     // windowed prefill: fewest query tokens of a sequence that are its work: 2, or
                       // 1 where no decode kernel is launched
-  int direct;         // windowed decode: 1 selects the direct schedule
+  int direct;         // windowed decode: 1 selects the direct schedule, 2 the same as workgroups
+                      // of the pair prefill's launch
   uint32_t last_block;  // windowed: the pool's last page, which an id outside the pool is read as
 };
 

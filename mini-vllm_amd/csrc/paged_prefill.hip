@@ -9,7 +9,9 @@
 // Three kernels: the pair kernel (further down, with its own schedule) for GQA pairs at D =
 // 128 over pages of at least 16 keys with a positive scale, which is every prefill of the 0.6B
 // shapes; paged_prefill_lds_kernel for odd groups at D = 128 over 16-bit pools; and
-// paged_prefill_kernel for the rest. Design of the latter two (this library's own):
+// paged_prefill_kernel for the rest. Windowed calls (a row sees the last `window` keys and the first
+// `sinks`) take the pair kernel at D = 128, for odd groups and fp8 pools too, and window_prefill.hip's
+// for the rest. Design of the latter two of the three (this library's own):
 //
 //  * work item = (sequence, column, query tile): 128 query positions of HW query heads
 //    (HW = 2 heads of one GQA group when the group is even) against one kv head. Its
@@ -56,13 +58,13 @@
 
 #include "common.hpp"
 #include "paged_attention.hpp"
+#include "paged_decode_rows.hpp"
 #include "window_list.hpp"
 
 namespace mvllm {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileKeys = kPrefillKeyTile;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -1384,11 +1386,18 @@ __global__ __launch_bounds__(256) void paged_prefill_lds_kernel(const PagedParam
 //
 // kOne (windowed, on the grid): the same for groups with an odd head: an item's waves are 32
 // positions each of one query head, twice the positions of a pair's item.
-template <typename TQ, typename TKV, int kWaves, bool kSplit, bool kWindow, bool kOne = false>
+//
+// kDecode (windowed): the batch's decode rows too, a workgroup per (sequence, chunk of kDecode query
+// heads), where they run on what the items leave idle instead of a launch before them: behind a
+// list's items, or on the item grid in place of the sequence's last query tile, which it does not
+// have. The waves' partial results meet in the first tile's buffers. With 20 decode rows of 1028
+// keys and a chunk of 512 tokens over fp8 48 us before, 34 beside; the launch's rule has the rest.
+template <typename TQ, typename TKV, int kWaves, bool kSplit, bool kWindow, bool kOne = false, int kDecode = 0>
 __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(const PagedParams p) {
   constexpr bool kFp8 = std::is_same_v<TKV, fp8_t>;
   constexpr int D = 128;
   static_assert(!kOne || (kWindow && !kSplit), "single heads: windowed items on the grid");
+  static_assert(kDecode == 0 || (kWindow && !kOne), "decode rows beside windowed items of pairs");
   constexpr int kHeads = kOne ? 1 : 2;
   constexpr int QT = kWaves * 32 / kHeads;   // query positions: kWaves / kHeads waves of 32 per head
   constexpr int KW = kTileKeys / kWaves;     // keys of a tile staged by one wave
@@ -1415,6 +1424,27 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(c
     if constexpr (decltype(par)::value == 0) return v_lds0; else return v_lds1;
   };
 
+  if constexpr (kDecode > 0) {
+    int seq = -1, unit = 0;
+    if constexpr (kSplit) {
+      const int row = static_cast<int>(blockIdx.x) - p.hq / 2 * p.pf_ranks, units = p.hq / kDecode;
+      if (row >= 0) {
+        seq = row / units;
+        unit = row % units;
+      }
+    } else if (blockIdx.z == gridDim.z - 1 && sload(p.seq_lens + blockIdx.y) == 1) {
+      if (static_cast<int>(blockIdx.x) >= p.hq / kDecode) return;
+      seq = blockIdx.y;
+      unit = blockIdx.x;
+    }
+    if (seq >= 0) {
+      static_assert(kWaves * kDecode * D * 4 <= kTileBytes && kWaves * kDecode * 8 <= kTileBytes,
+                    "the waves' partial results fit");
+      decode_list<TQ, TKV, D, kDecode, kWaves>(p, seq, unit, reinterpret_cast<float*>(k_lds0),
+                                               reinterpret_cast<float*>(v_lds0));
+      return;
+    }
+  }
   const int tid = threadIdx.x;
   const int wave = uniform(tid / kWave);
   const int lane = tid % kWave;
@@ -2154,6 +2184,24 @@ void launch_prefill_cfg(const PagedParams& p, int max_query_len, hipStream_t str
   }
 }
 
+// The pair kernel on `items`, and with the decode rows beside them where the plan says so (p.direct 2).
+template <typename TQ, typename TKV, int kWaves, bool kSplit, bool kWindow>
+void launch_pair_kernel(const PagedParams& p, dim3 items, hipStream_t stream) {
+  if constexpr (kWindow) {
+    if (p.direct == 2) {
+      const int chunk = decode_group_chunk(p.hq / p.hk);
+      if (kSplit) items.x += p.hq / chunk * p.num_seqs;
+      if (chunk == 4) {
+        paged_prefill_pair_kernel<TQ, TKV, kWaves, kSplit, true, false, 4><<<items, kWaves * kWave, 0, stream>>>(p);
+      } else {
+        paged_prefill_pair_kernel<TQ, TKV, kWaves, kSplit, true, false, 2><<<items, kWaves * kWave, 0, stream>>>(p);
+      }
+      return;
+    }
+  }
+  paged_prefill_pair_kernel<TQ, TKV, kWaves, kSplit, kWindow><<<items, kWaves * kWave, 0, stream>>>(p);
+}
+
 // The pair kernel by its schedule (pf_pieces >= 1: a workgroup per position of it; pieces
 // merged after) or on the item grid.
 template <typename TQ, typename TKV, int kWaves, bool kWindow>
@@ -2163,7 +2211,7 @@ void launch_prefill_ranked(const PagedParams& p, hipStream_t stream) {
   if (p.num_seqs > kWave) {
     paged_prefill_schedule_kernel<QT, std::is_same_v<TKV, fp8_t>, kWindow><<<1, kWave, 0, stream>>>(p);
   }
-  paged_prefill_pair_kernel<TQ, TKV, kWaves, true, kWindow><<<grid, kWaves * kWave, 0, stream>>>(p);
+  launch_pair_kernel<TQ, TKV, kWaves, true, kWindow>(p, grid, stream);
   if (p.pf_pieces > 1) {
     paged_prefill_pair_merge_kernel<TQ, QT><<<grid, kPairMergeThreads, 0, stream>>>(p);
   }
@@ -2179,11 +2227,11 @@ void launch_prefill_pair(const PagedParams& p, int max_query_len, hipStream_t st
   }
   if (p.pf_tile == 128) {
     const int wide = (max_query_len + 127) / 128;
-    paged_prefill_pair_kernel<TQ, TKV, 8, false, kWindow><<<dim3(cols, p.num_seqs, wide), 512, 0, stream>>>(p);
+    launch_pair_kernel<TQ, TKV, 8, false, kWindow>(p, dim3(cols, p.num_seqs, wide), stream);
     return;
   }
   const int qtiles = (max_query_len + 63) / 64;
-  paged_prefill_pair_kernel<TQ, TKV, 4, false, kWindow><<<dim3(cols, p.num_seqs, qtiles), 256, 0, stream>>>(p);
+  launch_pair_kernel<TQ, TKV, 4, false, kWindow>(p, dim3(cols, p.num_seqs, qtiles), stream);
 }
 
 template <typename TQ>

@@ -14,11 +14,12 @@
 // A 16-bit or float32 pool of the inputs' type takes the rows as rope then a copy give them, bit for
 // bit. An fp8 page keeps a power-of-two scale per kv head for K and for V, as kv_write.hip
 // describes (grown as the page fills, its rows re-encoded when it grows); K is quantised from the
-// float32 rotation, without a rounding to the inputs' type between. There a workgroup takes a run
-// (tokens on consecutive rows of one page) and one kv head: every thread a row's piece of K or of
-// V, the page's two maxima meet in LDS, and each row is rotated, scaled and stored by the thread
-// that loaded it. (One workgroup for a run's heads together, a thread walking the run's rows, as the
-// plain write has it, would hold a page's rotated rows in float32, 256 registers a thread.)
+// float32 rotation, without a rounding to the inputs' type between. There a workgroup takes a window of
+// tokens and one kv head, with the runs (tokens on consecutive rows of one page) that start in it: every
+// thread a row's piece of K or of V, a run's two maxima meet in LDS, and each row is rotated, scaled
+// and stored by the thread that loaded it. (One workgroup for a run's heads together, a thread walking
+// the run's rows, as the plain write has it, would hold a page's rotated rows in float32, 256 registers
+// a thread.)
 
 #include <algorithm>
 

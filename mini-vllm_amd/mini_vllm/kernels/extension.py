@@ -333,7 +333,7 @@ class _BlasChoice(ctypes.Structure):
 # ``mvllm_sampling_row`` of include/minivllm_hip.h: temperature, top_p, top_k.
 _SAMPLING_ROW = struct.Struct("@ffi")
 
-DECODE_MODES = {0: "none", 1: "stream", 2: "grid", 3: "by_row", 4: "direct"}
+DECODE_MODES = {0: "none", 1: "stream", 2: "grid", 3: "by_row", 4: "direct", 5: "beside"}
 
 
 def _bind(lib: ctypes.CDLL) -> None:

@@ -112,6 +112,29 @@ def test_decode_schedules(lib):
                                  {"decode_schedule": 4})
 
 
+def test_decode_rows_beside_the_prefill(lib):
+    """In the prefill's launch where their lists end within it; a launch of their own for long lists,
+    many of them, or shapes that the pair kernel does not take."""
+    def mode(n, tokens, window, chunk=512, **more):
+        return plan(lib, window=window, num_tokens=n + tokens, num_seqs=n + tokens // chunk,
+                    max_query_len=chunk, max_context_len=30000, **more)["decode_mode"]
+    fp8 = {"kv_dtype": torch.float8_e4m3fn}
+    assert mode(8, 512, 1024) == mode(8, 512, 1024, **fp8) == mode(62, 512, 1024) == "beside"
+    assert mode(100, 2048, 1024) == mode(1, 64, 1024, 64, **fp8) == mode(30, 2048, 2000) == "beside"
+    assert {mode(1, 64, 1024, 64), mode(31, 512, 4096), mode(250, 4096, 512), mode(16, 512, 2000),
+            mode(126, 4096, 1000, **fp8), mode(8, 512, 1024, head_dim=64)} <= {"direct", "stream"}
+    assert mode(8, 512, 1024, options={"decode_schedule": 4}) == "direct"
+    assert mode(31, 512, 4096, options={"decode_schedule": 5}) == "beside"
+    assert mode(8, 512, 1024, head_dim=64, options={"decode_schedule": 5}) in ("direct", "stream")
+    beside = plan(lib, window=256, num_tokens=520, num_seqs=9, max_query_len=512)
+    assert beside["decode_workgroups"] == 9 * 8
+    assert plan(lib, window=256, num_tokens=1024, num_seqs=2, max_query_len=512)["decode_mode"] == "none"
+    with pytest.raises(RuntimeError, match="out of range"):
+        plan(lib, options={"decode_schedule": 6})
+    with pytest.raises(RuntimeError, match="out of range"):
+        plan(lib, options={"decode_schedule": 3})
+
+
 def test_a_plan_goes_by_the_window_not_the_context(lib):
     # the fewest keys of a share at this type are 16: no more workgroups than shares of the window
     stream = {"decode_schedule": 1}

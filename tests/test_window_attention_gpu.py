@@ -124,6 +124,49 @@ def test_prefill_schedules(device, extension, chunks, kv_dtype, pieces, schedule
     assert_close(got, b)
 
 
+BESIDE = MIXED + DECODES + [(40, 0), (0, 1)]
+
+
+@pytest.mark.parametrize("dtype,kv_dtype", [x for x in TYPES if x[0] != torch.float32])
+@pytest.mark.parametrize("hq,hk", [(16, 8), (4, 1), (6, 1), (16, 2)])
+@pytest.mark.parametrize("schedule,pieces", [(1, 3), (2, 1), (0, 1)])
+@pytest.mark.parametrize("n", [1, 5])
+def test_decode_rows_beside_the_prefill(device, extension, n, schedule, pieces, hq, hk, dtype, kv_dtype):
+    """In the prefill's launch, behind listed items and on the item grid, up to 64 sequences and more."""
+    b = rolling_batch(BESIDE * n, 70, 9, dtype=dtype, kv_dtype=kv_dtype, hq=hq, hk=hk, spare_rows=3)
+    args = on(b, device)
+    options = {"decode_schedule": 5, "prefill_schedule": schedule, "prefill_pieces": pieces}
+    plan = extension.paged_window_attention_plan(
+        b["q"].shape[0], len(BESIDE) * n, hq, hk, 128, 16, b["max_query_len"], b["max_context_len"], 70, 9,
+        b["q"].dtype, b["key_pool"].dtype, options)
+    assert plan["decode_mode"] == "beside"
+    got = extension.paged_window_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], b["max_query_len"], b["max_context_len"], 70, 9,
+        b["scale"], args["k_scale"], args["v_scale"], plan_options=options)
+    assert_close(got, b)
+
+
+@pytest.mark.parametrize("n", [0, 70])
+def test_decode_rows_beside_items_of_128(device, extension, n):
+    pairs = [(600 - 7 * i, 512) for i in range(3)] + [(300, 1), (0, 1), (900, 1)] + [(9 + i, 1) for i in range(n)]
+    b = rolling_batch(pairs, 200, 5, dtype=torch.bfloat16, kv_dtype=torch.float8_e4m3fn, hq=32, hk=8)
+    plan = extension.paged_window_attention_plan(
+        b["q"].shape[0], len(pairs), 32, 8, 128, 16, 512, 900, 200, 5, torch.bfloat16, torch.float8_e4m3fn)
+    assert (plan["decode_mode"], plan["prefill_item"]) == ("beside", 128)
+    assert_close(call(b, device), b)
+
+
+def test_decode_rows_beside_a_prefill_without_a_positive_scale(device, extension):
+    b = rolling_batch(BESIDE, 70, 9, dtype=torch.bfloat16, hq=4, hk=2, scale=-0.2)
+    args = on(b, device)
+    got = extension.paged_window_attention(
+        args["q"], args["key_pool"], args["value_pool"], args["block_tables"], args["cu_seqlens_q"],
+        args["context_lens"], args["seq_lens"], b["max_query_len"], b["max_context_len"], 70, 9,
+        b["scale"], plan_options={"decode_schedule": 5})
+    assert_close(got, b)
+
+
 @pytest.mark.parametrize("staging", [0, 1])
 def test_long_window_of_a_long_context(device, extension, staging):
     b = rolling_batch([(9000, 100), (8200, 1)], 4100, 21, dtype=torch.bfloat16, hq=2, hk=1)
