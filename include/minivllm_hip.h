@@ -168,9 +168,10 @@ int mvllm_paged_attention(void* out, const void* q, const void* key_pool,
  *   A page holding no key that a query of the call sees is not read and its table entry may be
  * anything (-1: a rolling cache gives such pages to other sequences), and what the keys that no
  * query sees hold in a page that is read has no part in the result. K and V of a key that some
- * query sees must be finite. A visible key's entry outside [0, num_blocks) is read as the pool's last
- * page: the result is meaningless then, but nothing outside the pool is read. A decode row without a key (context_lens[s] <= 0) is zeros; rows of
- * out that belong to no sequence are left as they are. */
+ * query sees must be finite. A visible key's entry outside [0, num_blocks) is read as the pool's
+ * last page: the result is meaningless then, but nothing outside the pool is read. A decode row
+ * without a key (context_lens[s] <= 0) is zeros; rows of out that belong to no sequence are left as
+ * they are. */
 int mvllm_paged_window_attention_plan(int32_t num_tokens, int32_t num_seqs, int32_t num_q_heads,
                                       int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                                       int32_t max_query_len, int32_t max_context_len,

@@ -1390,8 +1390,8 @@ __global__ __launch_bounds__(256) void paged_prefill_lds_kernel(const PagedParam
 // kDecode (windowed): the batch's decode rows too, a workgroup per (sequence, chunk of kDecode query
 // heads), where they run on what the items leave idle instead of a launch before them: behind a
 // list's items, or on the item grid in place of the sequence's last query tile, which it does not
-// have. The waves' partial results meet in the first tile's buffers. With 20 decode rows of 1028
-// keys and a chunk of 512 tokens over fp8 48 us before, 34 beside; the launch's rule has the rest.
+// have. The waves' partial results meet in the first tile's buffers. 28 rows of up to 705 keys
+// and five chunks of 61 to 512 tokens over fp8: 48 us before, 34 beside; the planner's rule has more.
 template <typename TQ, typename TKV, int kWaves, bool kSplit, bool kWindow, bool kOne = false, int kDecode = 0>
 __global__ __launch_bounds__(kWaves * kWave, 2) void paged_prefill_pair_kernel(const PagedParams p) {
   constexpr bool kFp8 = std::is_same_v<TKV, fp8_t>;

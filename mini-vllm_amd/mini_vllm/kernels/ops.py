@@ -680,7 +680,8 @@ def paged_window_attention(
     v_scale: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """:func:`paged_attention` over a sliding window with sinks (no counterpart in the
-    reference). Kernels: the windowed forms of ``csrc/paged_{decode,prefill}.hip``.
+    reference). Kernels: the windowed forms of ``csrc/paged_{decode,prefill}.hip`` and
+    ``csrc/window_prefill.hip``.
 
     A query at position p (of a sequence of S keys computing L tokens, query r stands at
     S - L + r) sees the keys ``j <= p`` with ``j > p - window`` or ``j < sinks``: the ``window``
