@@ -435,6 +435,7 @@ bool beside_prefill(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk
       !pair_prefill(hq, hk, d, block_size, q_dtype, kv_dtype, o)) {
     return false;
   }
+  if (num_seqs * decode_units(hq, hk) > (1 << 20)) return false;  // (the launch's first extent)
   if (o.decode_schedule != 0) return o.decode_schedule == MVLLM_DECODE_BESIDE;
   const int cus = device_cus();
   const PairWork w = pair_work(num_tokens, num_seqs, hq, max_q, window_span(max_ctx, win), true);

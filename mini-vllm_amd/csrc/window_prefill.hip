@@ -1,7 +1,7 @@
 // Windowed prefill attention for the shapes that the pair kernel (paged_prefill.hip) does not take:
 // head dims 32, 64 and 256, and at 128 pages of fewer than 16 keys and a scale that is not positive;
-// any GQA group, 16-bit queries over a pool of their type or fp8. A query at position p sees the keys j <= p with
-// j > p - window or j < sinks.
+// any GQA group, 16-bit queries over a pool of their type or fp8. A query at position p sees the keys
+// j <= p with j > p - window or j < sinks.
 //
 // Design:
 //  * a work item is kRows rows of one (sequence, kv head), a row being one (query position, query
@@ -11,10 +11,10 @@
 //  * an item walks the entries of its key list (paged_attention.hpp): exactly the sinks and the
 //    keys from its first query's window to its last query, 64 a tile.
 //  * 4 waves of 32 rows (two blocks of 16, one K / V fragment read from LDS feeding the MFMAs of
-//    both), at D = 256 8 waves of 16, K and V row-major in LDS. S^T = K Q^T on v_mfma_f32_16x16x32: a lane holds one row's
-//    scores of keys 4 g + i of every 16 (g = lane / 16). The PV product sums over keys, so P^T is
-//    used as the scores lie: of a step of 32 keys a lane has 4 g .. 4 g + 3 and 16 + 4 g .. + 3, and
-//    V is read transposed (ds_read_b64_tr_b16) in that order.
+//    both), at D = 256 8 waves of 16, K and V row-major in LDS. S^T = K Q^T on v_mfma_f32_16x16x32:
+//    a lane holds one row's scores of keys 4 g + i of every 16 (g = lane / 16). The PV product sums
+//    over keys, so P^T is used as the scores lie: of a step of 32 keys a lane has 4 g .. 4 g + 3 and
+//    16 + 4 g .. + 3, and V is read transposed (ds_read_b64_tr_b16) in that order.
 //  * LDS chunks are swizzled by their row so that the rows that one read serves lie in distinct banks.
 //  * the next tile's rows are requested before a tile is computed and stored to LDS after it, into a
 //    second buffer; page ids one tile before that.
