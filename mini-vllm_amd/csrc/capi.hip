@@ -417,9 +417,9 @@ bool all_chunks(int32_t num_tokens, int32_t num_seqs, int32_t max_q) {
 
 // Windowed decode rows as workgroups of the pair prefill's launch, where they run on what the items
 // leave idle: instead of a launch or two before it, but with the prefill's 4 waves a list, two
-// workgroups a CU. Worth it while a list, 4.5 us and 22 bytes a ns (17 over fp8), ends within the
-// launches that it takes the place of (three quarters of a cut prefill, whose pieces leave no CU idle),
-// and while lists are not most of the work.
+// workgroups a CU. Worth it while a list, 4.5 us and 22 bytes a ns (17 over fp8, 18 with the products
+// of 4 heads), ends within the launches that it takes the place of (less of a cut prefill, whose
+// pieces leave no CU idle), and while lists are not most of the work.
 // Before and beside, us, rows of window 1024 but where said and a chunk of 512: bf16, 8 rows 44 and 29,
 // 31 53 and 35, 62 and a chunk of 256 74 and 69, 100 and four chunks 120 and 109, 20 and 8 of 256 52 and
 // 43, 30 (window 2048) and four 94 and 79; fp8, 48 and 36, 50 and 45, 60 and 54, 104 and 94, 61 and 43,
@@ -427,6 +427,9 @@ bool all_chunks(int32_t num_tokens, int32_t num_seqs, int32_t max_q) {
 // What the rule leaves out: that over bf16, 30 and 33; 16 rows of 2000 63 and 70; 31 of 4096 127 and
 // 133, over fp8 106 and 112; 4 of 4096 and a chunk of 1024 90 and 118, 92 and 107; and with eight chunks
 // 250 rows of 512 130 and 135, 108 and 148, over fp8 126 rows of 1000 114 and 145.
+//   With 4 query heads a kv head, bf16: 8 and a chunk of 512 57 and 47, 62 and 256 81 and 73; left out,
+// 120 and 256 130 and 171, 20 rows and a chunk of 16 42 and 50. Where three workgroups and more read
+// each kv head (24 heads over 4): 62 rows and 256 88 and 75, left out 60 rows of 2000 132 and 173.
 constexpr int kBesideKeys = 2048;
 bool beside_prefill(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int32_t d, int32_t block_size,
                     int32_t max_q, int32_t max_ctx, int32_t keys, int32_t q_dtype, int32_t kv_dtype,
@@ -443,15 +446,17 @@ bool beside_prefill(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk
   const int64_t lists = (num_seqs - w.chunks) * decode_units(hq, hk);
   const bool fp8 = kv_dtype == mvllm::kFP8E4M3;
   if (lists < 1 || keys > kBesideKeys || lists > 4 * cus) return false;
-  if (fp8 && lists > 2 * cus && lists + w.wgs > 5 * cus) return false;
+  const bool slow = !fp8 && mvllm::decode_group_chunk(hq / hk) == 4;
+  const bool thrice = decode_units(hq, hk) > 2 * hk;
+  if (lists > 2 * cus && (slow || (thrice && keys > 1200) || (fp8 && lists + w.wgs > 5 * cus))) return false;
   const mvllm::PairCosts c = mvllm::pair_costs(64, fp8);  // (in 10 ns)
   const double share = static_cast<double>(w.wgs) / cus;
   const double prefill = pair_mode(w, num_seqs, hq, max_q, kv_dtype, cus, true).cut
-                             ? 7.5 * (static_cast<double>(c.cut * w.n) * share + c.fixed)
-                             : 10.0 * static_cast<double>(c.whole * w.n) * (share > 1.0 ? share : 1.0);
+                             ? 7.0 * (static_cast<double>(c.cut * w.n) * share + c.fixed)
+                             : 11.0 * static_cast<double>(c.whole * w.n) * (share > 1.0 ? share : 1.0);
   const double list = 2.0 * static_cast<double>(keys) * d * element_bytes(kv_dtype);
   const double rows = 10e3 + list * static_cast<double>(lists) / 6200;
-  return 4.5e3 + list / (fp8 ? 17 : 22) <= prefill + rows;
+  return 4.5e3 + list / (fp8 ? 17 : (slow ? 18 : 22)) <= prefill + rows;
 }
 
 Plan make_plan(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int32_t d,
@@ -478,19 +483,35 @@ Plan make_plan(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int
   return plan;
 }
 
-// Windowed decode: the direct schedule or the stream, for lists of at most `keys` entries, from what
-// each was measured to take (us a call): direct 4.5 + a list at 34 bytes a ns (30 over fp8), the
-// stream 10 + all lists at 6.2 TB/s, while a CU has one list at most. Direct and stream, bf16, 8 kv
-// heads: one sequence of 64 keys 4.8 and 9.5, of 512 10.1 and 11.1, of 1024 17 and 11.5; 16 of 1024 19.2
-// and 19.2, of 2048 33 and 29; 28 of 1024 23 and 28.
+// Windowed decode: the direct schedule or the stream, for lists of at most `keys` entries by chunks of
+// `chunk` query heads, from what each was measured to take (us a call): direct 3.5 + a list at 34
+// bytes a ns (27 where a row is of at most 128 bytes, 26 with the products of 4 heads), the stream 11
+// (12 over fp8) + all lists at 6.2 TB/s, while a CU has one list at most; over fp8 with 4 heads 7 and
+// 20 bytes a ns, and 17. Direct and stream, bf16, 8 kv heads, 2 query heads each: one sequence of 64
+// keys 4.8 and 9.5, of 512 9.4 and 11.1, of 1024 15 and 11.5; 16 of 1024 18.9 and 19.2, of 2048 33
+// and 29; 28 of 1024 23 and 28; 4 query heads each: one of 512 14.5 and 13.1, 16 of 1024 25.5 and 23.9,
+// of 512 16.1 and 17.8; over fp8 one of 512 9.3 and 12.9, 16 of 2048 26 and 22; with 4 heads one of
+// 512 14.7 and 18.4, of 1024 21.5 and 19.3.
 //   Past that both run at the memory's rate and direct saves the second launch (64 of 1024 46 and
-// 49, 256 of 1024 169 and 174), but for fp8: rows of 128 bytes apart are read at 5 TB/s, the stream's
-// whole tokens at 6 (64 of 4096 112 and 96, 256 of 1024 109 and 97), so only short lists of not
-// too many (64 of 1024 31 and 32, 128 of 512 31 and 33).
-bool direct_decode(int64_t lists, int64_t keys, int64_t row_bytes, bool fp8, int cus) {
-  if (lists > cus) return !fp8 || (lists <= 4 * cus && keys <= 1024);
+// 49, 256 of 1024 169 and 174), but for rows of 128 bytes, which it reads at 5 TB/s, the stream's
+// whole tokens at 6 (fp8, 64 of 4096 112 and 96, 256 of 1024 109 and 97): only short lists of not
+// too many (64 of 1024 31 and 32, 128 of 512 31 and 33). Over fp8 with 4 heads up to two a CU (64 of
+// 1024 45.3 and 45.9, 128 87 and 76; of 64 bytes a row 41 and 31), and where each kv head is three
+// lists and more: 24 heads over 4, whose waves share a workgroup on the grid, 128 of 64 14 and 11, of
+// 1024 129 and 110; 12 over 2, on the stream, 128 of 64 8.6 and 13.6 but of 1024 65 and 60.
+bool direct_decode(int64_t lists, int64_t keys, int64_t row_bytes, bool fp8, int32_t hq, int32_t hk, int cus) {
+  const int chunk = mvllm::decode_group_chunk(hq / hk);
+  const bool narrow = row_bytes <= 128, slow = fp8 && chunk == 4;
+  if (lists > cus) {
+    const int64_t units = decode_units(hq, hk);
+    if (lists > 2 * cus && units > 2 * hk && (units > 8 || keys > 600)) return false;
+    if (slow) return lists <= 2 * cus && row_bytes >= 128;
+    return !narrow || (lists <= 4 * cus && keys <= 1024);
+  }
   const double list = 2.0 * static_cast<double>(keys * row_bytes);
-  return 4.5e3 + list / (fp8 ? 30 : 34) <= 10e3 + list * static_cast<double>(lists) / 6200;
+  const double rate = slow ? 20 : (chunk == 4 ? 26 : (narrow ? 27 : 34));
+  return (slow ? 7e3 : 3.5e3) + list / rate <=
+         (slow ? 17e3 : (fp8 ? 12e3 : 11e3)) + list * static_cast<double>(lists) / 6200;
 }
 
 void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk,
@@ -512,7 +533,7 @@ void plan_decode(Plan& plan, int32_t num_tokens, int32_t num_seqs, int32_t hq, i
              (o.decode_schedule == MVLLM_DECODE_DIRECT ||
               ((o.decode_schedule == 0 || o.decode_schedule == MVLLM_DECODE_BESIDE) &&
                direct_decode(num_seqs * units, max_ctx, static_cast<int64_t>(d) * element_bytes(kv_dtype),
-                             kv_dtype == mvllm::kFP8E4M3, device_cus())))) {
+                             kv_dtype == mvllm::kFP8E4M3, hq, hk, device_cus())))) {
     plan.pub.decode_mode = MVLLM_DECODE_DIRECT;
     plan.pub.decode_workgroups = static_cast<int32_t>(num_seqs * units);
     return;
