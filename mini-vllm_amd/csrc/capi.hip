@@ -490,13 +490,13 @@ Plan make_plan(int32_t num_tokens, int32_t num_seqs, int32_t hq, int32_t hk, int
 // 20 bytes a ns, and 17. Direct and stream, bf16, 8 kv heads, 2 query heads each: one sequence of 64
 // keys 4.8 and 9.5, of 512 9.4 and 11.1, of 1024 15 and 11.5; 16 of 1024 18.9 and 19.2, of 2048 33
 // and 29; 28 of 1024 23 and 28; 4 query heads each: one of 512 14.5 and 13.1, 16 of 1024 25.5 and 23.9,
-// of 512 16.1 and 17.8; over fp8 one of 512 9.3 and 12.9, 16 of 2048 26 and 22; with 4 heads one of
-// 512 14.7 and 18.4, of 1024 21.5 and 19.3.
+// of 512 16.1 and 17.8; over fp8 one of 512 8.8 and 11.5, of 1024 13.9 and 12.5; with 4 heads one of
+// 512 13.2 and 15.0, of 1024 20.6 and 15.8, 28 of 1024 22.5 and 32.
 //   Past that both run at the memory's rate and direct saves the second launch (64 of 1024 46 and
 // 49, 256 of 1024 169 and 174), but for rows of 128 bytes, which it reads at 5 TB/s, the stream's
 // whole tokens at 6 (fp8, 64 of 4096 112 and 96, 256 of 1024 109 and 97): only short lists of not
-// too many (64 of 1024 31 and 32, 128 of 512 31 and 33). Over fp8 with 4 heads up to two a CU (64 of
-// 1024 45.3 and 45.9, 128 87 and 76; of 64 bytes a row 41 and 31), and where each kv head is three
+// too many (64 of 1024 31 and 32, 128 of 512 31 and 33). Over fp8 with 4 heads up to two a CU (128
+// of 1024 83 and 74; of 64 bytes a row 64 and 47), and where each kv head is three
 // lists and more: 24 heads over 4, whose waves share a workgroup on the grid, 128 of 64 14 and 11, of
 // 1024 129 and 110; 12 over 2, on the stream, 128 of 64 8.6 and 13.6 but of 1024 65 and 60.
 bool direct_decode(int64_t lists, int64_t keys, int64_t row_bytes, bool fp8, int32_t hq, int32_t hk, int cus) {

@@ -318,7 +318,8 @@ __global__ __launch_bounds__(512) void paged_decode_stream_kernel(const PagedPar
                     score_scale, st);
         }
       }
-      K::merge_row_groups(st);
+      if constexpr (kWindow) K::sum_row_groups(st);
+      else K::merge_row_groups(st);
       if (g == 0) {
         if (whole) {
           K::write_output(p, row, h0, r, st);
@@ -500,7 +501,8 @@ __global__ __launch_bounds__(512) void paged_decode_grid_kernel(const PagedParam
     K::stream(p, table, 0, pages_in_lds ? s_pages : nullptr, first_page, kvh, sb, se, g, r, qf,
               p.scale * kLog2e, st);
   }
-  K::merge_row_groups(st);
+  if constexpr (kWindow) K::sum_row_groups(st);
+  else K::merge_row_groups(st);
   if (g != 0) return;
   if (nsplit == 1) {
     K::write_output(p, row, h0, r, st);
